@@ -431,6 +431,109 @@ MINICPMO_API int minicpmo_gpu_attention_no_alloc(const float *q, const void *k_c
                                     size_t pos, size_t head_count, size_t kv_head_count, size_t head_dim,
                                     size_t context_capacity, float *dst, void *stream, char *error, size_t error_cap);
 
+/* ---- paged serving operators (no reference counterpart) ----
+ * One serving step of requests that come and go, over caller-owned DEVICE
+ * buffers, without a context: plan gives every request's new tokens their
+ * pages, positions and cache slots; append writes their K and V rows there;
+ * attention attends them over the pages.  All calls enqueue on `stream` (a
+ * cudaStream_t, NULL for the legacy stream) without waiting for it, allocate
+ * nothing, read no device value on the host and can be captured into graphs.
+ * The buffers belong to the device that is current.  Return 1, or 0 with a
+ * message in `error`; the host checks come before any launch. */
+
+/* Most requests of one call. */
+#define MINICPMO_PAGED_MAX_REQUESTS 8192
+/* Bytes of the attention's workspace, whatever the shapes. */
+#define MINICPMO_PAGED_WORKSPACE_BYTES (64u << 20)
+
+/* The pages of one layer's K and V caches: the row of position p of a
+ * request, kv head h, starts at element page * page_stride + (p % page_size)
+ * * token_stride + h * head_stride of each, page = table[p / page_size].
+ * Rows are head_dim contiguous values; either order of tokens and heads
+ * within a page.  Base pointers and strides are multiples of 16 bytes. */
+typedef struct minicpmo_paged_cache {
+    void *k, *v;
+    int dtype;            /* F32 = 0, F16 = 1, BF16 = 20 */
+    uint32_t page_size;   /* positions per page: a power of two in 8..256 */
+    uint32_t kv_heads;
+    uint32_t head_dim;    /* 64, 128 or 256 */
+    uint64_t n_pages;
+    uint64_t page_stride, token_stride, head_stride; /* elements */
+} minicpmo_paged_cache;
+
+/* plan: one scheduler step of n_req requests.  lens[r] positions of request
+ * r are cached; new_lens[r] >= 0 tokens join them now, -1 says that r is
+ * finished.  block_table is [n_req][max_pages] (rows table_stride entries
+ * apart): entry j of row r is the page of positions [j * page_size, ...).
+ * free_ring[ring_capacity] holds the free pages' ids: those at ring_state[0]
+ * (head) up to ring_state[1] (tail), both counting up forever, modulo
+ * ring_capacity.  The requests' new pages are taken at the head, in request
+ * order, and written behind the pages that their table rows hold; finished
+ * requests' pages join at the tail in the same order (they serve from the
+ * next call on), and their rows stay as they are.
+ * Outputs: lens_out and ring_state_out (may be lens and ring_state
+ * themselves); cu_new[n_req + 1], the prefix sums of the new tokens; for
+ * token t of request r, positions[t] = lens[r] + t - cu_new[r] and
+ * slots[t] = page * page_size + offset; slots -1 and positions 0 for the
+ * rest of token_capacity.  status[0]: 0, or why the step was refused (sum of
+ * 1: too few free pages; 2: a request longer than its table row; 4: more
+ * tokens than token_capacity; 8: a negative length, or new_lens below -1;
+ * 16: an inconsistent ring); then lens_out and ring_state_out repeat the
+ * inputs, block_table and free_ring are untouched, cu_new is all zero and
+ * every slot -1, so that append and attention of the same step do nothing.
+ * status[1]: free pages afterwards. */
+MINICPMO_API int minicpmo_gpu_paged_plan(const int32_t *lens, const int32_t *new_lens, size_t n_req, int32_t *block_table,
+                            size_t max_pages, size_t table_stride, int32_t *free_ring, size_t ring_capacity,
+                            const int64_t *ring_state, size_t page_size, size_t token_capacity, int32_t *lens_out,
+                            int64_t *ring_state_out, int32_t *cu_new, int32_t *positions, int64_t *slots,
+                            int32_t *status, void *stream, char *error, size_t error_cap);
+
+/* append: for each of n_tokens tokens with a slot >= 0, the K row of every
+ * kv head after RMSNorm over the head (k_norm[head_dim], f32; NULL: none)
+ * and RoPE (pairs (d, d + head_dim / 2), tables rope_cos / rope_sin
+ * [rope_context][head_dim / 2], f32) at positions[t], and the V row as it
+ * is, go to position slot % page_size of page slot / page_size.  With
+ * q_heads > 0 the token's q heads, normed with q_norm and rotated the same
+ * way, go to q_out[t] ([n_tokens][q_heads][head_dim], tokens q_out_stride
+ * elements apart).  Tokens whose slot is negative are left out, their q_out
+ * rows too.  q, k, v are in_dtype (F32, F16 or BF16), heads contiguous,
+ * tokens q_stride / k_stride / v_stride elements apart; the arithmetic is
+ * f32, rounded once to the cache's type, which is q_out's too.  Each slot at
+ * most once per call.  status (may be NULL): a device word that gets 1 added
+ * by OR for a position outside the tables, 2 for a slot outside the cache;
+ * those tokens are left out as well. */
+MINICPMO_API int minicpmo_gpu_paged_append(const minicpmo_paged_cache *cache, const void *q, const void *k, const void *v,
+                              int in_dtype, size_t n_tokens, size_t q_heads, size_t q_stride, size_t k_stride,
+                              size_t v_stride, const float *q_norm, const float *k_norm, float eps,
+                              const float *rope_cos, const float *rope_sin, size_t rope_context,
+                              const int32_t *positions, const int64_t *slots, void *q_out, size_t q_out_stride,
+                              int32_t *status, void *stream, char *error, size_t error_cap);
+
+/* attention: the new tokens of every request over its pages.  Token t of
+ * request r (cu_new[r] <= t < cu_new[r + 1]; cu_new is clamped to 0..n_tokens)
+ * stands at position p = lens[r] - (cu_new[r + 1] - t), lens counting the new
+ * tokens, and its q head h gets
+ *   out[t][h] = sum_{i <= p} softmax_i(scale * q[t][h] . K[i]) V[i]
+ * over the rows of kv head h / (q_heads / kv_heads); what lies behind p or
+ * behind the request's length is never used, whatever it holds.  A token with
+ * p < 0 sees nothing: its out rows are zero.  lse (may be NULL):
+ * [n_tokens][q_heads] f32, the natural logarithm of the softmax's
+ * denominator, -inf where nothing is seen.  q and out have the cache's type,
+ * heads contiguous, tokens q_stride / out_stride elements apart; rows at
+ * cu_new[n_req] and behind it are left as they are.  q_heads is a multiple of
+ * kv_heads, at most 16 per kv head.  Table entries outside the cache read as
+ * rows of zeros.  Scores, softmax statistics and sums are f32; for F16 and
+ * BF16 the softmax weights are rounded to the cache's type for the product
+ * with V.  workspace: MINICPMO_PAGED_WORKSPACE_BYTES, zero before its first
+ * use, 256-byte aligned; each call leaves it ready for the next.  Calls that
+ * may overlap on the GPU (streams, graphs replayed side by side) need one
+ * each. */
+MINICPMO_API int minicpmo_gpu_paged_attention(const minicpmo_paged_cache *cache, const void *q, size_t n_tokens,
+                                 size_t q_heads, size_t q_stride, const int32_t *block_table, size_t max_pages,
+                                 size_t table_stride, const int32_t *lens, const int32_t *cu_new, size_t n_req,
+                                 float scale, void *out, size_t out_stride, float *lse, void *workspace,
+                                 void *stream, char *error, size_t error_cap);
+
 #ifdef __cplusplus
 }
 #endif

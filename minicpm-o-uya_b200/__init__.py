@@ -9,6 +9,8 @@ This package is the Python mirror of the reference host side above that ABI:
   quantisers used to build seeded synthetic models
 * :mod:`.qwen3` -- the Qwen3 runtime mirroring ``src/minicpmo/qwen3.uya``
   (open runtime, tokenwise prefill, greedy generate, bench)
+* :mod:`.paged` -- paged serving operators on torch CUDA tensors: page
+  planning, the K/V append and attention over the pages
 
 There is no CPU fallback: if the helper library is missing or no B200 is
 present, the entry points raise.

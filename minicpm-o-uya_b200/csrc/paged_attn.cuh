@@ -1,0 +1,188 @@
+// paged_attn.cuh -- the work split of the paged attention kernels.
+//
+// A unit of work is one tile of KT keys for one block of new tokens of one
+// request and one kv head (all q heads of the group are rows of the block, so
+// K and V are read once for them).  The units of all requests, in the order
+// request, kv head, block, tile, are cut into equal contiguous ranges, one per
+// CTA: ragged lengths leave no CTA with more than one unit above the average,
+// whatever the mix of long and short requests, and the lengths stay on the
+// device.  A block whose tiles lie in several ranges is computed in pieces;
+// each piece leaves its sums in the workspace, and the CTA that finishes last
+// adds them in the ranges' order, so the result does not depend on timing.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+namespace mcpo {
+
+constexpr int kPagedMaxCtas = 1024;  // tickets in the workspace
+constexpr int kPagedMaxGroup = 16;   // q heads per kv head
+
+struct PagedAttnArgs {
+  const void* q;
+  void* out;
+  float* lse;
+  const void *kc, *vc;
+  const int32_t *table, *lens, *cu;
+  long long q_stride, out_stride, table_stride, page_stride, token_stride, head_stride;
+  int n_tokens, n_req, q_heads, kv_heads, group;
+  long long max_pages, n_pages;
+  int page_shift;
+  float scale_log2;     // scale * log2(e): scores are kept in base 2
+  unsigned* tickets;    // [kPagedMaxCtas], zero at rest
+  float* partial;       // [CTA][2][rows of a block][head_dim + 2]
+};
+
+// One request's share of the batch.
+struct PagedReq {
+  int q0, n_new, len, blocks;
+};
+
+__device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs& a, int r, int block_tokens) {
+  PagedReq q;
+  const int c0 = a.cu[r], c1 = a.cu[r + 1], len = a.lens[r];
+  q.q0 = min(max(c0, 0), a.n_tokens);
+  q.n_new = min(max(c1, q.q0), a.n_tokens) - q.q0;
+  const long long most = a.max_pages << a.page_shift;
+  q.len = (int)min((long long)max(len, 0), most);
+  q.blocks = (q.n_new + block_tokens - 1) / block_tokens;
+  return q;
+}
+
+// Keys that the last token of block b sees, and its tiles (at least one, so
+// that blocks that see nothing are written too).
+__device__ __forceinline__ int paged_seen(const PagedReq& q, int b, int block_tokens) {
+  const int last = min(q.n_new, (b + 1) * block_tokens) - 1;
+  return max(0, q.len - q.n_new + last + 1);
+}
+template <int KT>
+__device__ __forceinline__ int paged_tiles(const PagedReq& q, int b, int block_tokens) {
+  return max(1, (paged_seen(q, b, block_tokens) + KT - 1) / KT);
+}
+template <int KT>
+__device__ __forceinline__ long long paged_head_units(const PagedReq& q, int block_tokens) {
+  long long u = 0;
+  for (int b = 0; b < q.blocks; ++b) u += paged_tiles<KT>(q, b, block_tokens);
+  return u;
+}
+
+struct PagedShared {
+  long long red[32];
+  long long total, before;  // all units; those before request r
+  int r;                    // the request of this CTA's first unit
+};
+
+// A piece of one block: tiles [tile0, tile1) of n_tiles.
+struct PagedPiece {
+  PagedReq req;
+  int r, h, b, tile0, tile1, n_tiles;
+  int first_cta, n_ctas;  // the CTAs that share the block
+};
+
+template <int KT>
+struct PagedWalk {
+  const PagedAttnArgs& a;
+  int block_tokens, ctas;
+  long long total, u, u1;  // this CTA's next and last unit
+  PagedReq req;
+  int r, h, b;
+  long long block0;  // unit of the block's first tile
+
+  __device__ __forceinline__ long long first_unit(int cta) const { return (long long)cta * total / ctas; }
+  __device__ __forceinline__ int cta_of(long long unit) const { return (int)(((unit + 1) * ctas - 1) / total); }
+
+  // Block-wide: every thread of the CTA calls it, and gets the same walk.
+  __device__ PagedWalk(const PagedAttnArgs& args, PagedShared* s, int block_tokens_, int min_units)
+      : a(args), block_tokens(block_tokens_) {
+    const int n = a.n_req, nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (n + nt - 1) / nt, r0 = min(n, tid * per), r1 = min(n, r0 + per);
+    long long mine = 0;
+    for (int i = r0; i < r1; ++i) mine += paged_head_units<KT>(paged_req(a, i, block_tokens), block_tokens);
+    mine *= a.kv_heads;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) s->red[warp] = incl;
+    __syncthreads();
+    long long base = 0, all = 0;
+    for (int w = 0; w < nt / 32; ++w) {
+      if (w < warp) base += s->red[w];
+      all += s->red[w];
+    }
+    total = all;
+    ctas = (int)max(1ll, min((long long)gridDim.x, total / min_units));
+    u = blockIdx.x < (unsigned)ctas ? first_unit(blockIdx.x) : total;
+    u1 = blockIdx.x < (unsigned)ctas ? first_unit(blockIdx.x + 1) : total;
+    // the thread whose requests hold unit u walks to the one that has it
+    const long long ex = base + incl - mine;
+    if (u < u1 && u >= ex && u < ex + mine) {
+      long long at = ex;
+      for (int i = r0; i < r1; ++i) {
+        const long long ui = paged_head_units<KT>(paged_req(a, i, block_tokens), block_tokens) * a.kv_heads;
+        if (u < at + ui) {
+          s->r = i;
+          s->before = at;
+          break;
+        }
+        at += ui;
+      }
+    }
+    __syncthreads();
+    if (u < u1) {
+      r = s->r;
+      req = paged_req(a, r, block_tokens);
+      const long long off = u - s->before, per_head = paged_head_units<KT>(req, block_tokens);
+      h = (int)(off / per_head);
+      b = 0;
+      block0 = s->before + h * per_head;
+      while (u >= block0 + paged_tiles<KT>(req, b, block_tokens)) block0 += paged_tiles<KT>(req, b++, block_tokens);
+    }
+  }
+
+  // The next piece of this CTA's range; false at its end.
+  __device__ bool next(PagedPiece* p) {
+    if (u >= u1) return false;
+    const int n = paged_tiles<KT>(req, b, block_tokens);
+    p->req = req;
+    p->r = r;
+    p->h = h;
+    p->b = b;
+    p->n_tiles = n;
+    p->tile0 = (int)(u - block0);
+    p->tile1 = (int)min((long long)n, u1 - block0);
+    p->first_cta = cta_of(block0);
+    p->n_ctas = cta_of(block0 + n - 1) - p->first_cta + 1;
+    u = block0 + p->tile1;
+    if (p->tile1 == n && u < u1) {
+      block0 = u;
+      if (++b == req.blocks) {
+        b = 0;
+        if (++h == a.kv_heads) {
+          h = 0;
+          do {
+            req = paged_req(a, ++r, block_tokens);
+          } while (req.blocks == 0);
+        }
+      }
+    }
+    return true;
+  }
+};
+
+// The workspace slot of CTA `cta`'s piece of a block that begins in
+// first_cta: a CTA holds at most one block that began before it (0) and one
+// that goes on behind it (1).
+__device__ __forceinline__ long long paged_slot(int cta, int first_cta) { return 2ll * cta + (cta == first_cta ? 1 : 0); }
+
+__device__ __forceinline__ float paged_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace mcpo

@@ -72,6 +72,23 @@ class Qwen3Config(C.Structure):
     ]
 
 
+class PagedCache(C.Structure):
+    """minicpmo_paged_cache of include/minicpmo_gpu.h."""
+
+    _fields_ = [
+        ("k", vp),
+        ("v", vp),
+        ("dtype", i32),
+        ("page_size", u32),
+        ("kv_heads", u32),
+        ("head_dim", u32),
+        ("n_pages", C.c_uint64),
+        ("page_stride", C.c_uint64),
+        ("token_stride", C.c_uint64),
+        ("head_stride", C.c_uint64),
+    ]
+
+
 REFERENCE_SYMBOLS = (
     "minicpmo_gpu_context_create",
     "minicpmo_gpu_context_destroy",
@@ -155,6 +172,15 @@ SIGNATURES = {
     "minicpmo_gpu_context_qwen3_step_trace": (i32, [vp, vp, sz, u32ptr, u32ptr]),
     "minicpmo_gpu_context_qwen3_graph_trace": (i32, [vp, vp, sz, u32ptr, u32ptr]),
     "minicpmo_gpu_attention_no_alloc": (i32, [vp, vp, vp, i32, sz, sz, sz, sz, sz, vp, vp] + E),
+    "minicpmo_gpu_paged_plan": (i32, [vp, vp, sz, vp, sz, sz, vp, sz, vp, sz, sz, vp, vp, vp, vp, vp, vp, vp] + E),
+    "minicpmo_gpu_paged_append": (
+        i32,
+        [C.POINTER(PagedCache), vp, vp, vp, i32, sz, sz, sz, sz, sz, vp, vp, f32, vp, vp, sz, vp, vp, vp, sz, vp, vp] + E,
+    ),
+    "minicpmo_gpu_paged_attention": (
+        i32,
+        [C.POINTER(PagedCache), vp, sz, sz, sz, vp, sz, sz, vp, vp, sz, f32, vp, sz, vp, vp, vp] + E,
+    ),
 }
 
 
