@@ -534,6 +534,30 @@ MINICPMO_API int minicpmo_gpu_paged_attention(const minicpmo_paged_cache *cache,
                                  float scale, void *out, size_t out_stride, float *lse, void *workspace,
                                  void *stream, char *error, size_t error_cap);
 
+/* sample: one token per row of device logits [rows][vocab] (dtype F32, F16 or
+ * BF16, rows `stride` elements apart), from given uniform random numbers.
+ * With x the logits, T the row's temperature and w_i = exp((x_i - max x) / T):
+ * the tokens are ordered by x, equal ones by index; of that order the
+ * shortest of these prefixes is kept, at least one token: the first top_k;
+ * the first whose weights reach top_p of all tokens' weights (the full
+ * softmax, not what top_k left); the tokens with w_i >= min_p.  The draw is
+ * the first token whose running sum of weights reaches uniform times the
+ * kept sum.  Parameters are device arrays [rows] (NULL: off): temperature
+ * (NULL: 1; up to 1e-6 or NaN: greedy, the first largest logit), top_k (0 or
+ * less: off), top_p (0.999999 or more, or NaN: off), min_p (0 or less, or
+ * NaN: off); uniform in [0, 1], clamped, NaN as 0.  NaN logits count as -inf;
+ * tokens at -inf are never kept; where +inf occurs those tokens share the
+ * weight.  A row with nothing above -inf gets token 0, probability 0, kept 0.
+ * Outputs [rows]: tokens; probs (may be NULL), the token's weight over the
+ * kept sum; kept (may be NULL), the number of tokens kept.  Weights are
+ * computed in 64 bits and added as integers, so ranks and sums do not depend
+ * on the order of execution.  vocab at most 2^19.  No workspace; stream,
+ * capture and device as for the paged calls. */
+MINICPMO_API int minicpmo_gpu_sample(const void *logits, int dtype, size_t rows, size_t vocab, size_t stride,
+                        const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                        const float *uniform, int32_t *tokens, float *probs, int32_t *kept, void *stream, char *error,
+                        size_t error_cap);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,7 +26,7 @@ inline int paged_error(char* err, size_t cap, const char* fmt, ...) {
 // Bytes of one value of an activation or cache type; 0: not one of them.
 inline size_t paged_type_bytes(int dtype) { return dtype == kF32 ? 4 : dtype == kF16 || dtype == kBF16 ? 2 : 0; }
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+__host__ __device__ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Whether p is memory of the current device (or managed memory).
 bool paged_on_device(const void* p, const char* op, char* err, size_t cap);

@@ -172,6 +172,7 @@ SIGNATURES = {
     "minicpmo_gpu_context_qwen3_step_trace": (i32, [vp, vp, sz, u32ptr, u32ptr]),
     "minicpmo_gpu_context_qwen3_graph_trace": (i32, [vp, vp, sz, u32ptr, u32ptr]),
     "minicpmo_gpu_attention_no_alloc": (i32, [vp, vp, vp, i32, sz, sz, sz, sz, sz, vp, vp] + E),
+    "minicpmo_gpu_sample": (i32, [vp, i32, sz, sz, sz, vp, vp, vp, vp, vp, vp, vp, vp, vp] + E),
     "minicpmo_gpu_paged_plan": (i32, [vp, vp, sz, vp, sz, sz, vp, sz, vp, sz, sz, vp, vp, vp, vp, vp, vp, vp] + E),
     "minicpmo_gpu_paged_append": (
         i32,

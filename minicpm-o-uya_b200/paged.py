@@ -217,3 +217,37 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
           cu_new.data_ptr(), n, hd ** -0.5 if scale is None else scale, out.data_ptr(), os, _ptr(lse),
           workspace.data_ptr())
     return out
+
+
+class Sampled(NamedTuple):
+    token: torch.Tensor  # int32 [rows]
+    prob: torch.Tensor   # f32 [rows]: the token's share of the kept weights
+    kept: torch.Tensor   # int32 [rows]: tokens that the filters kept
+
+
+def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+           top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+           min_p: Optional[torch.Tensor] = None, out: Optional[Sampled] = None) -> Sampled:
+    """One token per row of logits [rows, vocab] (f32, f16 or bf16) from uniform random numbers f32 [rows]
+    (``minicpmo_gpu_sample``): temperature, top_p, min_p f32 [rows] and top_k int32 [rows], each None for off."""
+    op = "sample"
+    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in _DTYPES or logits.stride(1) != 1:
+        raise GpuError(f"error: {op}: logits must be a [rows, vocab] f32, f16 or bf16 CUDA tensor with contiguous rows")
+    dev, (n, vocab) = logits.device, logits.shape
+    f32 = torch.float32
+    _tensor(op, "uniform", uniform, dev, f32, (n,))
+    for name, t, dtype in (("temperature", temperature, f32), ("top_k", top_k, torch.int32), ("top_p", top_p, f32),
+                           ("min_p", min_p, f32)):
+        if t is not None:
+            _tensor(op, name, t, dev, dtype, (n,))
+    if out is None:
+        words = torch.empty(3, n, dtype=torch.int32, device=dev)
+        out = Sampled(words[0], words[1].view(f32), words[2])
+    else:
+        _tensor(op, "out.token", out.token, dev, torch.int32, (n,))
+        _tensor(op, "out.prob", out.prob, dev, f32, (n,))
+        _tensor(op, "out.kept", out.kept, dev, torch.int32, (n,))
+    _call(lib().minicpmo_gpu_sample, dev, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab,
+          logits.stride(0) if n > 1 else vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+          uniform.data_ptr(), out.token.data_ptr(), out.prob.data_ptr(), out.kept.data_ptr())
+    return out
