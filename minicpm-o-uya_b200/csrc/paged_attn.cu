@@ -245,6 +245,355 @@ __global__ void __launch_bounds__(kSimtThreads) k_paged_attn_f32(const PagedAttn
   }
 }
 
+// ---------------------------------------------------------------------
+// f16, bf16: few rows per request (decode, speculated tokens)
+// ---------------------------------------------------------------------
+// HBM-bound: K and V of a request are read once for the up to 16 rows (tokens
+// x q heads of the group) of a block, and 16 rows are one m16n8k16 tile, so
+// the legacy matrix instructions are far from their limit.  Each of the four
+// warps takes 16 of a tile's 64 keys with its own ring of cp.async stages, its
+// own maximum, sum and accumulator: nothing in the key loop waits on another
+// warp; the four join once per piece.  16 keys lie in one page (two for pages
+// of 8), so one table entry, fetched a tile ahead, addresses a warp's rows.
+constexpr int kMmaRows = 16, kMmaWarps = 4, kMmaKeys = 16, kMmaTile = kMmaWarps * kMmaKeys, kMmaThreads = kMmaWarps * 32;
+
+template <int HD>
+struct MmaCfg {
+  static constexpr int kStages = HD == 64 ? 6 : 3;
+  static constexpr int kTileBytes = kMmaKeys * HD * 2;  // a warp's K (or V) rows of one stage
+  static constexpr int kSmem = kMmaWarps * kStages * 2 * kTileBytes;
+  static constexpr int kCtas = HD == 256 ? 1 : 2;  // per SM
+};
+
+template <typename T>
+struct Frag;
+template <>
+struct Frag<__half> {
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+  static constexpr uint32_t kExp = 0x7c007c00u;  // exponent bits of both values
+};
+template <>
+struct Frag<__nv_bfloat16> {
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+  static constexpr uint32_t kExp = 0x7f807f80u;
+};
+
+// Whether either 16-bit value of u is infinite or NaN.
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint32_t u) {
+  const uint32_t e = u & Frag<T>::kExp;
+  return (e & 0xffffu) == (Frag<T>::kExp & 0xffffu) || (e >> 16) == (Frag<T>::kExp >> 16);
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kMmaThreads, MmaCfg<HD>::kCtas) k_paged_attn_mma(const PagedAttnArgs a) {
+  using Cfg = MmaCfg<HD>;
+  constexpr int kChunks = HD / 8;                      // 16-byte chunks of a row
+  constexpr int kCopies = kMmaKeys * kChunks / 32;     // of a lane, per K (or V) tile
+  constexpr int kStages = Cfg::kStages;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ PagedShared sched;
+  __shared__ unsigned last_s;
+  __shared__ float stat_s[kMmaWarps][2][kMmaRows];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r4 = lane >> 2, c4 = lane & 3;
+  uint8_t* ring = smem_raw + warp * kStages * 2 * Cfg::kTileBytes;
+  const uint32_t ring_a = smem_addr(ring);
+  const int block_tokens = kMmaRows / a.group;
+  PagedWalk<kMmaTile> walk(a, &sched, block_tokens, 1);
+  PagedPiece p;
+  while (walk.next(&p)) {
+    const int t0 = p.b * block_tokens, rows = min(block_tokens, p.req.n_new - t0) * a.group;
+    const int seen = paged_seen(p.req, p.b, block_tokens);
+    const int n_tiles = p.tile1 - p.tile0, key_first = p.tile0 * kMmaTile + warp * kMmaKeys;
+    const int32_t* table = a.table + p.r * a.table_stride;
+    const T* kg = static_cast<const T*>(a.kc) + p.h * a.head_stride;
+    const T* vg = static_cast<const T*>(a.vc) + p.h * a.head_stride;
+    // the pages of a warp's 16 keys of tile i: rows 0-7 and 8-15
+    auto ids = [&](int i, int& id0, int& id1) {
+      const int key = key_first + i * kMmaTile;
+      id0 = i < n_tiles && key < seen ? table[key >> a.page_shift] : -1;
+      id1 = i < n_tiles && key + 8 < seen ? table[(key + 8) >> a.page_shift] : -1;
+    };
+    auto load = [&](int i, int id0, int id1) {
+      if (i < n_tiles) {
+        const int key0 = key_first + i * kMmaTile;
+        const uint32_t dst = ring_a + (i % kStages) * 2 * Cfg::kTileBytes;
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) {
+          const int e = lane + 32 * j, row = e / kChunks, c = e % kChunks;
+          const int id = row < 8 ? id0 : id1;
+          const bool in = key0 + row < seen && id >= 0 && id < a.n_pages;
+          const long long at =
+              in ? id * a.page_stride + ((key0 + row) & ((1 << a.page_shift) - 1)) * a.token_stride + c * 8 : 0;
+          const uint32_t d = dst + row * HD * 2 + ((c ^ (row & 7)) << 4);
+          const int n = in ? 16 : 0;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(kg + at), "r"(n) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + Cfg::kTileBytes), "l"(vg + at), "r"(n)
+                       : "memory");
+        }
+      }
+      cp_async_commit();
+    };
+    int id0, id1;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      ids(i, id0, id1);
+      load(i, id0, id1);
+    }
+    ids(kStages - 1, id0, id1);
+
+    uint32_t qf[HD / 16][4];
+    int see[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = r4 + 8 * i;
+      see[i] = row < rows ? max(0, p.req.len - p.req.n_new + t0 + row / a.group + 1) : 0;
+      const T* qr = static_cast<const T*>(a.q) + (p.req.q0 + t0 + row / a.group) * a.q_stride +
+                    (long long)(p.h * a.group + row % a.group) * HD + c4 * 2;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        qf[k][i] = row < rows ? *reinterpret_cast<const uint32_t*>(qr + k * 16) : 0u;
+        qf[k][2 + i] = row < rows ? *reinterpret_cast<const uint32_t*>(qr + k * 16 + 8) : 0u;
+      }
+    }
+    // keys that every row of the block sees: before them nothing is masked
+    const int see_all = max(0, p.req.len - p.req.n_new + t0 + 1);
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[HD / 8][4];
+#pragma unroll
+    for (int c = 0; c < HD / 8; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+
+    for (int i = 0; i < n_tiles; ++i) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      load(i + kStages - 1, id0, id1);  // into the stage that the last iteration read
+      ids(i + kStages, id0, id1);
+      const int key0 = key_first + i * kMmaTile;
+      if (key0 >= seen) continue;
+      const uint32_t kt = ring_a + (i % kStages) * 2 * Cfg::kTileBytes, vt = kt + Cfg::kTileBytes;
+      float sc[2][4] = {};
+      {
+        const int row = (lane & 7) + ((lane & 16) >> 1);  // matrices: keys 0-7 | 0-7 | 8-15 | 8-15, halves of 16 values
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          uint32_t b[4];
+          const int c = 2 * k + ((lane >> 3) & 1);
+          ldsm4(b, kt + row * HD * 2 + ((c ^ (row & 7)) << 4));
+          Frag<T>::mma(sc[0], qf[k], b[0], b[1]);
+          Frag<T>::mma(sc[1], qf[k], b[2], b[3]);
+        }
+      }
+      const bool partial = key0 + kMmaKeys > see_all;
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = sc[n][e] * a.scale_log2;
+          if (partial && key0 + n * 8 + c4 * 2 + (e & 1) >= see[e >> 1]) v = -INFINITY;
+          sc[n][e] = v;
+          mx[e >> 1] = fmaxf(mx[e >> 1], v);
+        }
+      float base[2], corr[2];
+      bool moved = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+        const float mn = fmaxf(m[r], mx[r]);
+        base[r] = mn == -INFINITY ? 0.f : mn;
+        corr[r] = paged_exp2(m[r] - base[r]);
+        moved |= mn > m[r];
+        m[r] = mn;
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) l[r] *= corr[r];
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          o[c][0] *= corr[0], o[c][1] *= corr[0];
+          o[c][2] *= corr[1], o[c][3] *= corr[1];
+        }
+      }
+      uint32_t pf[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = paged_exp2(sc[n][e] - base[e >> 1]);
+          l[e >> 1] += w[e];
+        }
+        pf[2 * n] = Frag<T>::pack(w[0], w[1]);
+        pf[2 * n + 1] = Frag<T>::pack(w[2], w[3]);
+      }
+      bool wild = false;
+      if (partial) {
+        // a key that a row does not see adds nothing, whatever V holds there;
+        // 0 * inf would, so a tile with such values goes another way
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) {
+          const uint4 v = *reinterpret_cast<const uint4*>(ring + (i % kStages) * 2 * Cfg::kTileBytes + Cfg::kTileBytes +
+                                                          (lane + 32 * j) * 16);
+          wild |= not_finite<T>(v.x) || not_finite<T>(v.y) || not_finite<T>(v.z) || not_finite<T>(v.w);
+        }
+        wild = __any_sync(0xffffffffu, wild);
+      }
+      if (!wild) {
+        const int row = lane & 15;  // matrices: keys 0-7 | 8-15 of 8 values, twice
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) {
+          uint32_t b[4];
+          const int ch = 2 * c + (lane >> 4);
+          ldsm4t(b, vt + row * HD * 2 + ((ch ^ (row & 7)) << 4));
+          Frag<T>::mma(o[2 * c], pf, b[0], b[1]);
+          Frag<T>::mma(o[2 * c + 1], pf, b[2], b[3]);
+        }
+      } else {
+        for (int key = 0; key < kMmaKeys; ++key) {
+          // the weights of rows r4 and r4 + 8 for this key, from the lane of the quad that has them
+          const int src = (lane & ~3) | ((key & 7) >> 1);
+          const float2 lo = Frag<T>::unpack(__shfl_sync(0xffffffffu, pf[key < 8 ? 0 : 2], src));
+          const float2 hi = Frag<T>::unpack(__shfl_sync(0xffffffffu, pf[key < 8 ? 1 : 3], src));
+          const float w0 = key & 1 ? lo.y : lo.x, w1 = key & 1 ? hi.y : hi.x;
+          const bool on0 = key0 + key < see[0], on1 = key0 + key < see[1];
+#pragma unroll
+          for (int c = 0; c < HD / 8; ++c) {
+            const float2 v = Frag<T>::unpack(*reinterpret_cast<const uint32_t*>(
+                ring + (i % kStages) * 2 * Cfg::kTileBytes + Cfg::kTileBytes + key * HD * 2 + ((c ^ (key & 7)) << 4) + c4 * 4));
+            if (on0) o[c][0] += w0 * v.x, o[c][1] += w0 * v.y;
+            if (on1) o[c][2] += w1 * v.x, o[c][3] += w1 * v.y;
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+
+    // the four warps' sums, on the largest of their maxima
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (c4 == 0) {
+        stat_s[warp][0][r4 + 8 * r] = m[r];
+        stat_s[warp][1][r4 + 8 * r] = l[r];
+      }
+    }
+    __syncthreads();  // every warp is done with its ring
+    float* osum = reinterpret_cast<float*>(smem_raw);  // [warp][row][HD + 4]
+    constexpr int kLd = HD + 4;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = r4 + 8 * r;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kMmaWarps; ++w) mm = fmaxf(mm, stat_s[w][0][row]);
+      const float f = paged_exp2(m[r] - (mm == -INFINITY ? 0.f : mm));
+      float* dst = osum + (warp * kMmaRows + row) * kLd + c4 * 2;
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c)
+        *reinterpret_cast<float2*>(dst + c * 8) = make_float2(o[c][2 * r] * f, o[c][2 * r + 1] * f);
+    }
+    __syncthreads();
+    // from here on a thread has HD / 8 columns of one row, in groups of 4
+    const int row = tid >> 3, col = (tid & 7) * 4;
+    float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < kMmaWarps; ++w) mm = fmaxf(mm, stat_s[w][0][row]);
+    const float mbase = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+    for (int w = 0; w < kMmaWarps; ++w) ll += stat_s[w][1][row] * paged_exp2(stat_s[w][0][row] - mbase);
+    float4 acc[HD / 32];
+#pragma unroll
+    for (int c = 0; c < HD / 32; ++c) {
+      acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kMmaWarps; ++w) {
+        const float4 v = *reinterpret_cast<const float4*>(osum + (w * kMmaRows + row) * kLd + col + 32 * c);
+        acc[c].x += v.x, acc[c].y += v.y, acc[c].z += v.z, acc[c].w += v.w;
+      }
+    }
+    bool write = p.n_ctas == 1;
+    if (!write) {
+      float* part = a.partial + (paged_slot(blockIdx.x, p.first_cta) * kMmaRows + row) * kLd;
+      if (row < rows) {
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) *reinterpret_cast<float4*>(part + 4 + col + 32 * c) = acc[c];
+        if (col == 0) *reinterpret_cast<float2*>(part) = make_float2(mm, ll);
+      }
+      if (paged_last(a, p, &last_s)) {
+        write = true;
+        if (row < rows) {
+          mm = -INFINITY, ll = 0.f;
+          for (int c = 0; c < p.n_ctas; ++c)
+            mm = fmaxf(mm, __ldcg(a.partial + (paged_slot(p.first_cta + c, p.first_cta) * kMmaRows + row) * kLd));
+          const float b = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+          for (int k = 0; k < p.n_ctas; ++k) {
+            const float* src = a.partial + (paged_slot(p.first_cta + k, p.first_cta) * kMmaRows + row) * kLd;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src));
+            const float f = paged_exp2(ml.x - b);
+            ll += ml.y * f;
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(src + 4 + col + 32 * c));
+              acc[c].x += v.x * f, acc[c].y += v.y * f, acc[c].z += v.z * f, acc[c].w += v.w * f;
+            }
+          }
+        }
+      }
+    }
+    if (write && row < rows) {
+      const bool any = p.req.len - p.req.n_new + t0 + row / a.group + 1 > 0;
+      const long long t = p.req.q0 + t0 + row / a.group;
+      const int head = p.h * a.group + row % a.group;
+      const float inv = any ? 1.0f / ll : 0.f;
+      T* dst = static_cast<T*>(a.out) + t * a.out_stride + (long long)head * HD + col;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint2 u = make_uint2(0u, 0u);
+        if (any) u = make_uint2(Frag<T>::pack(acc[c].x * inv, acc[c].y * inv), Frag<T>::pack(acc[c].z * inv, acc[c].w * inv));
+        *reinterpret_cast<uint2*>(dst + 32 * c) = u;
+      }
+      if (a.lse && col == 0)
+        a.lse[t * a.q_heads + head] = any ? 0.693147180559945309f * (mm + log2f(ll)) : -INFINITY;
+    }
+    __syncthreads();  // the next piece's loads overwrite the sums
+  }
+}
+
 template <typename K>
 cudaError_t big_smem(K kernel, size_t bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
@@ -267,6 +616,28 @@ cudaError_t launch_f32(const PagedAttnArgs& a, cudaStream_t st) {
   k_paged_attn_f32<HD><<<ctas < kPagedMaxCtas ? ctas : kPagedMaxCtas, kSimtThreads, sizeof(SimtSmem<HD>), st>>>(a);
   return cudaGetLastError();
 }
+
+template <typename T, int HD>
+cudaError_t launch_mma(const PagedAttnArgs& a, cudaStream_t st) {
+  using Cfg = MmaCfg<HD>;
+  static_assert(Cfg::kSmem >= kMmaWarps * kMmaRows * (HD + 4) * 4, "the joined sums fit the rings");
+  int sms = 0;
+  cudaError_t e = sm_count(&sms);
+  if (e == cudaSuccess) e = big_smem(k_paged_attn_mma<T, HD>, Cfg::kSmem);
+  if (e != cudaSuccess) return e;
+  const int ctas = Cfg::kCtas * sms;
+  k_paged_attn_mma<T, HD><<<ctas < kPagedMaxCtas ? ctas : kPagedMaxCtas, kMmaThreads, Cfg::kSmem, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_16(const PagedAttnArgs& a, int hd, cudaStream_t st) {
+  return hd == 64 ? launch_mma<T, 64>(a, st) : hd == 128 ? launch_mma<T, 128>(a, st) : launch_mma<T, 256>(a, st);
+}
+
+// the workspace holds two pieces of 16 rows for every CTA
+static_assert((size_t)kPagedMaxCtas * 4 + (size_t)kPagedMaxCtas * 2 * kMmaRows * 260 * 4 <= MINICPMO_PAGED_WORKSPACE_BYTES,
+              "workspace");
 
 }  // namespace
 }  // namespace mcpo
@@ -332,6 +703,10 @@ extern "C" int minicpmo_gpu_paged_attention(const minicpmo_paged_cache* cache, c
   cudaError_t e = cudaErrorNotSupported;
   if (cache->dtype == kF32)
     e = hd == 64 ? launch_f32<64>(a, st) : hd == 128 ? launch_f32<128>(a, st) : launch_f32<256>(a, st);
+  else if (cache->dtype == kF16)
+    e = launch_16<__half>(a, (int)hd, st);
+  else
+    e = launch_16<__nv_bfloat16>(a, (int)hd, st);
   if (e != cudaSuccess) return paged_error(error, error_cap, "error: %s: launch: %s", op, cudaGetErrorString(e));
   return 1;
 }

@@ -441,3 +441,88 @@ def test_attention_f32(pkg, case, heads_out):
     _check_attention(c, *first)
     again = _run_attention(paged, c, ws)  # the workspace is ready again, and the result does not move
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+CASES_16 = F32_CASES + [
+    (128, 32, 8, 16, [(565, 1)]), (128, 8, 2, 8, [(77, 1), (1, 1), (64, 64), (65, 65), (63, 2)]),
+    (128, 16, 1, 256, [(4096, 1), (17, 2)]), (64, 12, 4, 16, [(129, 129), (700, 5), (128, 128), (4, 4)]),
+    (256, 16, 2, 32, [(513, 3), (64, 1)]), (128, 28, 4, 64, [(900, 300), (257, 257), (2, 2)]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("case", range(len(CASES_16)))
+@pytest.mark.parametrize("heads_out", [False, True])
+def test_attention_16_bits(pkg, dtype, case, heads_out):
+    from minicpmo_b200 import paged
+
+    hd, heads, kv, page, reqs = CASES_16[case]
+    c = _attention_case(200 + case, dtype, hd, heads, kv, page, reqs, heads_out)
+    ws = paged.workspace()
+    first = _run_attention(paged, c, ws)
+    _check_attention(c, *first)
+    again = _run_attention(paged, c, ws)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd, heads, kv, reqs", [(128, 4, 2, [(40, 12), (300, 5)]), (64, 8, 8, [(600, 500)]),
+                                                 (128, 8, 1, [(300, 290), (170, 170)]), (256, 2, 2, [(90, 33)])])
+def test_values_behind_a_token_do_not_reach_it(pkg, dtype, hd, heads, kv, reqs):
+    """Infinities and NaN in the K and V rows of the newest tokens: tokens before them keep finite results, tokens from
+    them on get what the definition gives."""
+    from minicpmo_b200 import paged
+
+    c = _attention_case(7, dtype, hd, heads, kv, 16, reqs)
+    for r, (n, m) in enumerate(reqs):
+        row = lambda p: (int(c["table"][r, p // 16]), p % 16)  # noqa: E731
+        c["vc"][row(n - 1)][0, 3] = math.inf
+        c["vc"][row(n - 2)][kv - 1, 5] = math.nan
+        c["vc"][row(n - m + 1)][0, 0] = -math.inf
+        c["kc"][row(n - 1)][kv - 1, 2] = math.nan
+    ws = paged.workspace()
+    out, lse = _run_attention(paged, c, ws)
+    for r, (n, m) in enumerate(reqs):  # only the last token of each request meets the NaN key
+        assert torch.isnan(lse[c["cu"][r + 1] - 1, heads - 1]) and torch.isfinite(lse[c["cu"][r]:c["cu"][r + 1] - 1]).all()
+        assert torch.isfinite(out[c["cu"][r]]).all()
+    live = c["cu"][-1]
+    want, _, _ = attention_reference(c["q"][:live], c["kc"], c["vc"], c["table"], c["lens"], c["cu"], hd ** -0.5)
+    assert torch.equal(torch.isnan(out[:live]), torch.isnan(want))
+    inf = torch.isinf(want)
+    assert inf.any() and torch.equal(out[:live][inf].double(), want[inf])
+    assert torch.isfinite(out[:live][torch.isfinite(want)]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_bad_tables(pkg, dtype):
+    """Table entries outside the cache read as rows of zeros; prefix sums and lengths out of range are clamped."""
+    from minicpmo_b200 import paged
+
+    c = _attention_case(9, dtype, 128, 4, 2, 16, [(100, 1), (50, 20)])
+    c["table"][0, 2], c["table"][1, 1] = -3, c["kc"].shape[0]
+    out, lse = _run_attention(paged, c, paged.workspace())
+    zero = dict(c)
+    pages = c["kc"].shape[0]
+    zero["kc"], zero["vc"] = (torch.cat([x, torch.zeros_like(x[:1])]) for x in (c["kc"], c["vc"]))
+    zero["table"] = torch.where((c["table"] == -3) | (c["table"] == pages), pages, c["table"])
+    _check_attention(zero, out, lse)
+    c["cu"] = [-5, 21, c["T"] + 100]
+    c["lens"] = [10 ** 9, 60]
+    out, _ = _run_attention(paged, c, paged.workspace())
+    assert out.shape[0] == c["T"]
+
+
+@pytest.mark.gpu
+def test_negative_scale_and_one_workspace_for_many_shapes(pkg):
+    from minicpmo_b200 import paged
+
+    ws = paged.workspace()
+    for seed, (dtype, hd, heads, kv, page, reqs) in enumerate([
+            ("bf16", 128, 32, 8, 16, [(3000, 1)] * 3), ("f32", 64, 4, 4, 16, [(500, 2)]), ("f16", 64, 8, 2, 32, [(90, 90)] * 9),
+            ("bf16", 128, 32, 8, 64, [(1500, 700), (700, 700)]), ("f16", 256, 4, 1, 16, [(5000, 1)])]):
+        c = _attention_case(seed, dtype, hd, heads, kv, page, reqs)
+        for scale in (-0.05, 0.0, 0.11):
+            _check_attention(c, *_run_attention(paged, c, ws, scale), scale)
