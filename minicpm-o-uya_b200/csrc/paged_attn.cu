@@ -5,6 +5,7 @@
 //   m' = max(m, max_i s_i), l' = l 2^(m - m') + sum_i 2^(s_i - m'),
 //   o' = o 2^(m - m') + sum_i 2^(s_i - m') V_i;  out = o / l.
 // Pieces of the keys join the same way.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -13,6 +14,7 @@
 
 #include "paged.cuh"
 #include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
 #include "tma.cuh"
 
 namespace mcpo {
@@ -72,9 +74,10 @@ __global__ void __launch_bounds__(kSimtThreads) k_paged_attn_f32(const PagedAttn
   const float* qg = static_cast<const float*>(a.q);
   const float* kg = static_cast<const float*>(a.kc);
   const float* vg = static_cast<const float*>(a.vc);
-  PagedWalk<kSimtKeys> walk(a, &sched, block_tokens, 1);
+  PagedWalk<kSimtKeys> walk;
+  walk.start(a, &sched, block_tokens, 1);
   PagedPiece p;
-  while (walk.next(&p)) {
+  while (walk.next(a, &p)) {
     const int t0 = p.b * block_tokens, rows = min(block_tokens, p.req.n_new - t0) * a.group;
     const int seen = paged_seen(p.req, p.b, block_tokens);
     auto load = [&](int tile, int st) {
@@ -265,46 +268,6 @@ struct MmaCfg {
   static constexpr int kCtas = HD == 256 ? 1 : 2;  // per SM
 };
 
-template <typename T>
-struct Frag;
-template <>
-struct Frag<__half> {
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-  static __device__ __forceinline__ uint32_t pack(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
-  static constexpr uint32_t kExp = 0x7c007c00u;  // exponent bits of both values
-};
-template <>
-struct Frag<__nv_bfloat16> {
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-  static __device__ __forceinline__ uint32_t pack(float x, float y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  static __device__ __forceinline__ float2 unpack(uint32_t u) {
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-  }
-  static constexpr uint32_t kExp = 0x7f807f80u;
-};
-
-// Whether either 16-bit value of u is infinite or NaN.
-template <typename T>
-__device__ __forceinline__ bool not_finite(uint32_t u) {
-  const uint32_t e = u & Frag<T>::kExp;
-  return (e & 0xffffu) == (Frag<T>::kExp & 0xffffu) || (e >> 16) == (Frag<T>::kExp >> 16);
-}
-
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -330,9 +293,10 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<HD>::kCtas) k_paged_attn_m
   uint8_t* ring = smem_raw + warp * kStages * 2 * Cfg::kTileBytes;
   const uint32_t ring_a = smem_addr(ring);
   const int block_tokens = kMmaRows / a.group;
-  PagedWalk<kMmaTile> walk(a, &sched, block_tokens, 1);
+  PagedWalk<kMmaTile> walk;
+  walk.start(a, &sched, block_tokens, 1);
   PagedPiece p;
-  while (walk.next(&p)) {
+  while (walk.next(a, &p)) {
     const int t0 = p.b * block_tokens, rows = min(block_tokens, p.req.n_new - t0) * a.group;
     const int seen = paged_seen(p.req, p.b, block_tokens);
     const int n_tiles = p.tile1 - p.tile0, key_first = p.tile0 * kMmaTile + warp * kMmaKeys;
@@ -630,14 +594,82 @@ cudaError_t launch_mma(const PagedAttnArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
+// cuTensorMapEncodeTiled, from the driver.
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+
+// A 4-D map of 16-bit values read in boxes of 64 x box[0..2] with the
+// 128-byte swizzle; strides in values.
+bool encode4(CUtensorMap* m, bool bf16, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
+             const uint32_t (&box)[3]) {
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+  const cuuint64_t st[3] = {strides[0] * 2, strides[1] * 2, strides[2] * 2};
+  const cuuint32_t b[4] = {64, box[0], box[1], box[2]}, one[4] = {1, 1, 1, 1};
+  return encode_fn() &&
+         encode_fn()(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
+                     d, st, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// False where the driver does not take the strides: the other kernel does.
+bool tc_maps(TcMaps* m, const PagedAttnArgs& a, int hd, bool bf16) {
+  const uint64_t h = (uint64_t)hd, page = 1ull << a.page_shift, hs = a.head_stride, ts = a.token_stride, ps = a.page_stride;
+  const uint32_t rows = (uint32_t)(page < kTcKeys ? page : kTcKeys);
+  const uint64_t g = (uint64_t)a.group;
+  m->heads_inner = hs <= ts;
+  const uint64_t kd_h[4] = {h, (uint64_t)a.kv_heads, page, (uint64_t)a.n_pages}, ks_h[3] = {hs, ts, ps};
+  const uint64_t kd_t[4] = {h, page, (uint64_t)a.kv_heads, (uint64_t)a.n_pages}, ks_t[3] = {ts, hs, ps};
+  const uint32_t kb_h[3] = {1, rows, 1}, kb_t[3] = {rows, 1, 1};
+  for (int i = 0; i < 2; ++i) {
+    CUtensorMap* map = i ? &m->v : &m->k;
+    const void* base = i ? a.vc : a.kc;
+    if (!(m->heads_inner ? encode4(map, bf16, base, kd_h, ks_h, kb_h) : encode4(map, bf16, base, kd_t, ks_t, kb_t)))
+      return false;
+  }
+  const uint64_t qd[4] = {h, g, (uint64_t)a.kv_heads, (uint64_t)a.n_tokens}, qs[3] = {h, g * h, (uint64_t)a.q_stride};
+  const uint32_t qb[3] = {(uint32_t)g, 1, (uint32_t)(kTcRows / g)};
+  return encode4(&m->q, bf16, a.q, qd, qs, qb);
+}
+
+template <typename T, int HD>
+cudaError_t launch_tc(const PagedAttnArgs& a, const TcMaps& m, cudaStream_t st) {
+  int sms = 0;
+  cudaError_t e = sm_count(&sms);
+  if (e == cudaSuccess) e = big_smem(k_paged_attn_tc<T, HD>, TcCfg<HD>::kSmem);
+  if (e != cudaSuccess) return e;
+  k_paged_attn_tc<T, HD><<<sms < kTcMaxCtas ? sms : kTcMaxCtas, kTcThreads, TcCfg<HD>::kSmem, st>>>(a, m);
+  return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t launch_16(const PagedAttnArgs& a, int hd, cudaStream_t st) {
+  // Many rows per request: 256-row blocks on the tensor cores.  Few: 16-row
+  // blocks, whose time is the K/V stream's.
+  if (hd <= 128 && a.scale_log2 > 0.f && (long long)a.n_tokens * a.group >= 64ll * a.n_req) {
+    TcMaps m;
+    if (tc_maps(&m, a, hd, Frag<T>::kExp == 0x7f807f80u))
+      return hd == 64 ? launch_tc<T, 64>(a, m, st) : launch_tc<T, 128>(a, m, st);
+  }
   return hd == 64 ? launch_mma<T, 64>(a, st) : hd == 128 ? launch_mma<T, 128>(a, st) : launch_mma<T, 256>(a, st);
 }
 
-// the workspace holds two pieces of 16 rows for every CTA
-static_assert((size_t)kPagedMaxCtas * 4 + (size_t)kPagedMaxCtas * 2 * kMmaRows * 260 * 4 <= MINICPMO_PAGED_WORKSPACE_BYTES,
-              "workspace");
+// the workspace: tickets, the error word, then two pieces of a block for every CTA
+constexpr size_t kHeadBytes = kPagedMaxCtas * sizeof(unsigned) + 256;
+static_assert(kHeadBytes + (size_t)kPagedMaxCtas * 2 * kMmaRows * 260 * 4 <= MINICPMO_PAGED_WORKSPACE_BYTES, "workspace");
+static_assert(kHeadBytes + (size_t)kTcMaxCtas * 2 * 256 * 132 * 4 <= MINICPMO_PAGED_WORKSPACE_BYTES, "workspace");
+static_assert(2 * kTcMaxCtas <= kPagedMaxCtas, "tickets");
 
 }  // namespace
 }  // namespace mcpo
@@ -698,7 +730,8 @@ extern "C" int minicpmo_gpu_paged_attention(const minicpmo_paged_cache* cache, c
   a.page_shift = __builtin_ctz(cache->page_size);
   a.scale_log2 = (float)((double)scale * 1.4426950408889634074);
   a.tickets = static_cast<unsigned*>(workspace);
-  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kPagedMaxCtas * sizeof(unsigned));
+  a.err = reinterpret_cast<int*>(a.tickets + kPagedMaxCtas);
+  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeadBytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaErrorNotSupported;
   if (cache->dtype == kF32)

@@ -11,6 +11,8 @@
 // adds them in the ranges' order, so the result does not depend on timing.
 #pragma once
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -32,6 +34,7 @@ struct PagedAttnArgs {
   int page_shift;
   float scale_log2;     // scale * log2(e): scores are kept in base 2
   unsigned* tickets;    // [kPagedMaxCtas], zero at rest
+  int* err;             // raised by a bounded wait that gave up
   float* partial;       // [CTA][2][rows of a block][head_dim + 2]
 };
 
@@ -83,7 +86,6 @@ struct PagedPiece {
 
 template <int KT>
 struct PagedWalk {
-  const PagedAttnArgs& a;
   int block_tokens, ctas;
   long long total, u, u1;  // this CTA's next and last unit
   PagedReq req;
@@ -94,8 +96,8 @@ struct PagedWalk {
   __device__ __forceinline__ int cta_of(long long unit) const { return (int)(((unit + 1) * ctas - 1) / total); }
 
   // Block-wide: every thread of the CTA calls it, and gets the same walk.
-  __device__ PagedWalk(const PagedAttnArgs& args, PagedShared* s, int block_tokens_, int min_units)
-      : a(args), block_tokens(block_tokens_) {
+  __device__ __forceinline__ void start(const PagedAttnArgs& a, PagedShared* s, int block_tokens_, int min_units) {
+    block_tokens = block_tokens_;
     const int n = a.n_req, nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (n + nt - 1) / nt, r0 = min(n, tid * per), r1 = min(n, r0 + per);
     long long mine = 0;
@@ -145,7 +147,7 @@ struct PagedWalk {
   }
 
   // The next piece of this CTA's range; false at its end.
-  __device__ bool next(PagedPiece* p) {
+  __device__ __forceinline__ bool next(const PagedAttnArgs& a, PagedPiece* p) {
     if (u >= u1) return false;
     const int n = paged_tiles<KT>(req, b, block_tokens);
     p->req = req;
@@ -183,6 +185,47 @@ __device__ __forceinline__ float paged_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// What the kernels of 16-bit types need to know of them.
+template <typename T>
+struct Frag;
+template <>
+struct Frag<__half> {
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+  static constexpr uint32_t kExp = 0x7c007c00u;  // exponent bits of both values
+};
+template <>
+struct Frag<__nv_bfloat16> {
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+  static constexpr uint32_t kExp = 0x7f807f80u;
+};
+
+// Whether either 16-bit value of u is infinite or NaN.
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint32_t u) {
+  const uint32_t e = u & Frag<T>::kExp;
+  return (e & 0xffffu) == (Frag<T>::kExp & 0xffffu) || (e >> 16) == (Frag<T>::kExp >> 16);
 }
 
 }  // namespace mcpo

@@ -1,0 +1,574 @@
+// paged_attn_tc.cuh -- paged attention on the tcgen05 tensor cores, for
+// chunks of many new tokens (f16 or bf16, head_dim 64 or 128).
+//
+// A block is two tiles of 128 rows (tokens x q heads of a kv head).  Per tile
+// of 128 keys, S = Q K^T goes to tensor memory (128 f32 columns), one thread
+// per row turns it into weights P that overwrite the first 64 columns as
+// 16-bit values, and O += P V reads them from there.  Roles: warps 0-3 and 4-7
+// are the softmax of tile 0 and 1, warp 8 issues the MMAs, warp 9 the TMA
+// loads of Q and of K and V pages (a ring of 128-key stages that both tiles
+// read).  The MMAs are issued P V (0), Q K^T (0), P V (1), Q K^T (1), ...: while
+// one tile's softmax runs, the tensor cores have the other tile's products.
+//
+// Rows keep the maximum they began with until a score exceeds it by 2^8;
+// weights up to 2^8 lose nothing in these types, and the accumulator is
+// rescaled only then.  Tensor memory: S/P of the tiles in columns 0 and 128,
+// O in 256 and 256 + head_dim.
+#pragma once
+
+#include <cuda.h>
+
+#include "paged_attn.cuh"
+#include "tcgen05.cuh"
+#include "tma.cuh"
+
+namespace mcpo {
+
+constexpr int kTcRows = 128, kTcKeys = 128, kTcThreads = 320;
+constexpr int kTcMaxCtas = 240;  // by the workspace
+constexpr uint32_t kTcTmem = 512;
+
+template <int HD>
+struct TcCfg {
+  static constexpr int kStageBytes = kTcKeys * HD * 2;
+  static constexpr int kStages = HD == 128 ? 4 : 8;
+  static constexpr int kHalves = HD / 64;  // 128-byte column blocks of a row
+  static constexpr int kQBytes = kTcRows * HD * 2;
+  static constexpr int kSmem = 2 * kQBytes + kStages * kStageBytes + 1024;  // with slack for the 1 KB alignment
+};
+
+struct TcMaps {
+  CUtensorMap q, k, v;
+  int heads_inner;  // K/V map's dimensions: (hd, heads, tokens, pages), else (hd, tokens, heads, pages)
+};
+
+// K-major operand, 128-byte swizzle: rows of 128 bytes, 8-row groups 1 KB apart.
+__device__ __forceinline__ uint64_t tc_desc_k(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// MN-major operand, 128-byte swizzle: rows (k) of 64 values, 8-row groups 1 KB
+// apart, the next 64 values `lbo` bytes further.
+__device__ __forceinline__ uint64_t tc_desc_mn(uint32_t saddr, uint32_t lbo) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// 32 consecutive columns of this thread's lane; wait with tc_wait_ld before use.
+__device__ __forceinline__ void tc_ld32(uint32_t addr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_ld16(uint32_t addr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// Makes the registers of the loads above depend on the wait.
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tc_tma_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_addr(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ uint64_t f2_pack(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 f2_unpack(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+struct TcShared {
+  uint64_t q_full, q_empty;
+  uint64_t kv_full[8], kv_empty[8];
+  uint64_t s_full[2], p_full[2], o_full[2], epi_done[2];
+  uint32_t tmem;
+  int abort_;
+  unsigned last[2];
+  // Values of V that are not finite, in tiles that some row sees only part of:
+  // they are 0 for the product, and here is, per column, the first key that
+  // holds +inf, -inf or NaN.
+  int wild;
+  int first[3][128];
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    k_paged_attn_tc(const PagedAttnArgs a, const __grid_constant__ TcMaps maps) {
+  using Cfg = TcCfg<HD>;
+  constexpr int kStages = Cfg::kStages, kHalves = Cfg::kHalves, kLd = HD + 4;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ TcShared s;
+  __shared__ PagedShared sched;
+  uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  const uint32_t q_a = smem_addr(smem), kv_a = q_a + 2 * Cfg::kQBytes;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* abort_s = &s.abort_;
+
+  if (tid == 0) {
+    mbar_init(&s.q_full, 1);
+    mbar_init(&s.q_empty, 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(&s.kv_full[i], 1), mbar_init(&s.kv_empty[i], 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s.s_full[t], 1);
+      mbar_init(&s.p_full[t], 4);
+      mbar_init(&s.o_full[t], 1);
+      mbar_init(&s.epi_done[t], 4);
+    }
+    s.abort_ = 0;
+    s.wild = 0;
+    mbar_fence_init();
+  }
+  if (warp == 8) tmem_alloc(&s.tmem, kTcTmem);
+  const int tile_tokens = kTcRows / a.group, block_tokens = 2 * tile_tokens;
+  // every warp walks the CTA's pieces by itself, its lane 0 for it, with the
+  // state in shared memory: the softmax rows need the registers
+  __shared__ PagedWalk<kTcKeys> walks[kTcThreads / 32];
+  __shared__ PagedPiece pieces[kTcThreads / 32];
+  {
+    PagedWalk<kTcKeys> walk;
+    walk.start(a, &sched, block_tokens, 1);  // has barriers: the inits above are seen behind them
+    if (lane == 0) walks[warp] = walk;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem;
+  const PagedPiece& p = pieces[warp];
+  auto next_piece = [&]() -> bool {
+    __syncwarp();
+    bool more = false;
+    if (lane == 0) more = walks[warp].next(a, &pieces[warp]);
+    return __shfl_sync(0xffffffffu, (int)more, 0) != 0;
+  };
+
+  if (warp == 9) {
+    // ---- loads: one lane per box (a page's rows x 64 values) ----
+    const int box_rows = min(1 << a.page_shift, kTcKeys);
+    const int page_of = lane / kHalves, half = lane % kHalves;  // this lane's box of a stage
+    uint32_t stage_n = 0, piece_n = 0;
+    bool ok = true;
+    while (ok && next_piece()) {
+      const int t0 = p.b * block_tokens, seen = paged_seen(p.req, p.b, block_tokens);
+      const bool two = p.req.n_new - t0 > tile_tokens;
+      if (piece_n) ok = __all_sync(0xffffffffu, gwait(&s.q_empty, (piece_n - 1) & 1, a.err, abort_s));
+      if (!ok) break;
+      if (lane == 0) {
+        const uint32_t bytes = (uint32_t)(tile_tokens * a.group * HD * 2);
+        mbar_arrive_expect_tx(&s.q_full, two ? 2 * bytes : bytes);
+        for (int t = 0; t < (two ? 2 : 1); ++t)
+          for (int c = 0; c < kHalves; ++c)
+            tc_tma_4d(q_a + t * Cfg::kQBytes + c * (kTcRows * 128), &maps.q, c * 64, 0, p.h,
+                      p.req.q0 + t0 + t * tile_tokens, &s.q_full);
+      }
+      ++piece_n;
+      const int32_t* table = a.table + p.r * a.table_stride;
+      for (int i = p.tile0; ok && i < p.tile1; ++i) {
+        const int key0 = i * kTcKeys, left = min(kTcKeys, seen - key0);  // keys that the block sees
+        const int n = left > 0 ? (left + box_rows - 1) / box_rows : 0;
+        int id = 0;
+        if (page_of < n) {
+          id = table[(key0 + page_of * box_rows) >> a.page_shift];
+          if (id < 0 || id >= a.n_pages) id = (int)a.n_pages;  // out of the map: zeros
+        }
+        const int row = key0 & ((1 << a.page_shift) - 1);  // of pages longer than a tile
+        for (int kv = 0; kv < 2; ++kv, ++stage_n) {
+          const uint32_t st = stage_n % kStages;
+          if (stage_n >= kStages) ok = gwait(&s.kv_empty[st], (stage_n / kStages - 1) & 1, a.err, abort_s);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&s.kv_full[st], (uint32_t)(n * kHalves * box_rows * 128));
+          __syncwarp();
+          if (page_of < n) {
+            const uint32_t dst = kv_a + st * Cfg::kStageBytes + half * (kTcKeys * 128) + page_of * box_rows * 128;
+            const CUtensorMap* m = kv ? &maps.v : &maps.k;
+            if (maps.heads_inner) tc_tma_4d(dst, m, half * 64, p.h, row, id, &s.kv_full[st]);
+            else tc_tma_4d(dst, m, half * 64, row, p.h, id, &s.kv_full[st]);
+          }
+        }
+      }
+    }
+    // copies in flight land before the shared memory goes
+    __syncwarp();
+    if (lane == 0) {
+      if (piece_n) mbar_wait(&s.q_full, (piece_n - 1) & 1, a.err);
+      for (uint32_t i = stage_n > kStages ? stage_n - kStages : 0; i < stage_n; ++i)
+        mbar_wait(&s.kv_full[i % kStages], (i / kStages) & 1, a.err);
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    // ---- MMAs ----
+    if (lane == 0) {
+      constexpr uint32_t kType = sizeof(T) == 2 && Frag<T>::kExp == 0x7f807f80u ? 1u : 0u;  // 1: bf16
+      constexpr uint32_t kBase = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(kTcRows >> 4) << 24);
+      constexpr uint32_t kDescS = kBase | ((uint32_t)(kTcKeys >> 3) << 17);
+      constexpr uint32_t kDescO = kBase | (1u << 16) | ((uint32_t)(HD >> 3) << 17);  // V is MN-major
+      uint32_t stage_n = 0, piece_n = 0, p_n[2] = {0, 0}, epi_n[2] = {0, 0};
+      bool ok = true;
+      auto qk = [&](int t, uint32_t st) {
+        const uint32_t qa = q_a + t * Cfg::kQBytes, ka = kv_a + st * Cfg::kStageBytes;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t off = (k >> 2) * (kTcRows * 128) + (k & 3) * 32;
+          tc_mma_ss(tmem + t * 128, tc_desc_k(qa + off), tc_desc_k(ka + off), kDescS, k != 0);
+        }
+        umma_commit(&s.s_full[t]);
+      };
+      auto pv = [&](int t, uint32_t st, bool first) {
+        const uint32_t va = kv_a + st * Cfg::kStageBytes;
+#pragma unroll
+        for (int k = 0; k < kTcKeys / 16; ++k)
+          tc_mma_ts(tmem + 256 + t * HD, tmem + t * 128 + k * 8, tc_desc_mn(va + k * 2048, kTcKeys * 128), kDescO,
+                    !first || k != 0);
+      };
+      while (ok && walks[warp].next(a, &pieces[warp])) {
+        const int nt = p.req.n_new - p.b * block_tokens > tile_tokens ? 2 : 1, n = p.tile1 - p.tile0;
+        // the softmax warps have read the last block's O
+        for (int t = 0; t < 2; ++t)
+          if (epi_n[t]) ok = ok && gwait(&s.epi_done[t], (epi_n[t] - 1) & 1, a.err, abort_s);
+        ok = ok && gwait(&s.q_full, piece_n & 1, a.err, abort_s);
+        uint32_t ks = stage_n % kStages;
+        ok = ok && gwait(&s.kv_full[ks], (stage_n / kStages) & 1, a.err, abort_s);
+        if (!ok) break;
+        ++piece_n;
+        tc_fence_after();
+        for (int t = 0; t < nt; ++t) qk(t, ks);
+        umma_commit(&s.kv_empty[ks]);
+        if (n == 1) umma_commit(&s.q_empty);
+        for (int i = 0; ok && i < n; ++i) {
+          const uint32_t vn = stage_n + 2 * i + 1, kn = vn + 1, vs = vn % kStages;
+          ks = kn % kStages;
+          ok = gwait(&s.kv_full[vs], (vn / kStages) & 1, a.err, abort_s);
+          for (int t = 0; ok && t < nt; ++t) {
+            ok = gwait(&s.p_full[t], p_n[t] & 1, a.err, abort_s);
+            if (!ok) break;
+            ++p_n[t];
+            tc_fence_after();
+            pv(t, vs, i == 0);
+            if (t == nt - 1) umma_commit(&s.kv_empty[vs]);
+            if (i + 1 == n) {
+              umma_commit(&s.o_full[t]);
+            } else {
+              if (t == 0) ok = gwait(&s.kv_full[ks], (kn / kStages) & 1, a.err, abort_s);
+              if (!ok) break;
+              tc_fence_after();
+              qk(t, ks);
+              if (t == nt - 1) {
+                umma_commit(&s.kv_empty[ks]);
+                if (i + 2 == n) umma_commit(&s.q_empty);
+              }
+            }
+          }
+        }
+        stage_n += 2 * n;
+        for (int t = 0; t < nt; ++t) ++epi_n[t];
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax of tile t: thread = row ----
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_t = tmem + lane_base + t * 128, o_t = tmem + lane_base + 256 + t * HD;
+    uint32_t s_n = 0, o_n = 0, stage_n = 0;
+    bool ok = true;
+    while (ok && next_piece()) {
+      const int t0 = p.b * block_tokens, n = p.tile1 - p.tile0;
+      const int rows = min(tile_tokens, p.req.n_new - t0 - t * tile_tokens) * a.group;
+      if (rows <= 0) {
+        stage_n += 2 * n;
+        continue;
+      }
+      const int tok = t0 + t * tile_tokens + row / a.group;  // of the request's new tokens
+      const bool valid = row < rows;
+      // rows without a token see everything: what they compute is dropped
+      const int see = valid ? max(0, p.req.len - p.req.n_new + tok + 1) : INT_MAX;
+      const int see_all = max(0, p.req.len - p.req.n_new + t0 + 1);  // of the block's first token
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < n; ++i) {
+        const int key0 = (p.tile0 + i) * kTcKeys;
+        ok = __all_sync(0xffffffffu, gwait(&s.s_full[t], s_n & 1, a.err, abort_s));
+        if (!ok) break;
+        ++s_n;
+        tc_fence_after();
+        float x[kTcKeys];
+#pragma unroll
+        for (int c = 0; c < kTcKeys; c += 32) tc_ld32(s_t + c, x + c);
+        tc_wait_ld();
+#pragma unroll
+        for (int c = 0; c < kTcKeys; ++c) asm volatile("" : "+f"(x[c]));
+        if (t == 0 && key0 + kTcKeys > see_all) {
+          // some row sees only part of this tile: V must be finite where weights are 0
+          const uint32_t vn = stage_n + 2 * i + 1, vs = vn % kStages;
+          ok = __all_sync(0xffffffffu, gwait(&s.kv_full[vs], (vn / kStages) & 1, a.err, abort_s));
+          if (!ok) break;
+          uint8_t* v = smem + 2 * Cfg::kQBytes + vs * Cfg::kStageBytes;
+          if (i == 0 || key0 <= see_all) {  // the piece's first such tile
+            for (int e = tid; e < 3 * 128; e += 128) s.first[e / 128][e % 128] = INT_MAX;
+            if (tid == 0) s.wild = 0;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+          }
+          const int end = paged_seen(p.req, p.b, block_tokens) - key0;
+          for (int e = tid; e < Cfg::kStageBytes / 16; e += 128) {
+            uint4 u = *reinterpret_cast<const uint4*>(v + e * 16);
+            if (not_finite<T>(u.x) || not_finite<T>(u.y) || not_finite<T>(u.z) || not_finite<T>(u.w)) {
+              const int key = (e >> 3) % kTcKeys, half = (e >> 3) / kTcKeys, col = half * 64 + (((e & 7) ^ (key & 7)) << 3);
+              uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const uint32_t bits = (w[k >> 1] >> (16 * (k & 1))) & 0xffffu, ex = Frag<T>::kExp & 0xffffu;
+                if ((bits & ex) != ex) continue;
+                w[k >> 1] &= k & 1 ? 0x0000ffffu : 0xffff0000u;
+                if (key >= end) continue;  // behind the request: nobody sees it
+                const int kind = (bits & 0x7fffu) != ex ? 2 : bits >> 15;
+                atomicMin(&s.first[kind][col + k], key0 + key);
+                s.wild = 1;
+              }
+              *reinterpret_cast<uint4*>(v + e * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        if (__any_sync(0xffffffffu, key0 + kTcKeys > see)) {
+          const int lim = see - key0;
+#pragma unroll
+          for (int c = 0; c < kTcKeys; ++c) x[c] = c < lim ? x[c] : -INFINITY;
+        }
+        float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int c = 4; c < kTcKeys; c += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], c + 4 + k < kTcKeys ? fmaxf(x[c + k], x[c + 4 + k]) : x[c + k]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+        const bool up = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
+        float f = 1.0f;
+        if (up) {
+          f = paged_exp2(m - top);
+          m = top;
+          l *= f;
+        }
+        if (i > 0 && __any_sync(0xffffffffu, up)) {
+          // Q K^T of this tile was issued behind P V of the last one, so O is complete
+#pragma unroll
+          for (int c = 0; c < HD; c += 16) {
+            float o[16];
+            tc_ld16(o_t + c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              asm volatile("" : "+f"(o[k]));
+              o[k] *= f;
+            }
+            tc_st16(o_t + c, reinterpret_cast<const uint32_t*>(o));
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2), mb2 = f2_pack(-base, -base);
+        uint64_t sum[2] = {f2_pack(l, 0.f), f2_pack(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < kTcKeys; c += 64) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float2 y = f2_unpack(f2_fma(f2_pack(x[c + 2 * k], x[c + 2 * k + 1]), sc2, mb2));
+            const float w0 = paged_exp2(y.x), w1 = paged_exp2(y.y);
+            sum[k & 1] = f2_add(sum[k & 1], f2_pack(w0, w1));
+            pk[k] = Frag<T>::pack(w0, w1);
+          }
+          tc_st32(s_t + c / 2, pk);
+        }
+        const float2 s0 = f2_unpack(sum[0]), s1 = f2_unpack(sum[1]);
+        l = (s0.x + s0.y) + (s1.x + s1.y);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.p_full[t]);
+      }
+      stage_n += 2 * n;
+      if (!ok) break;
+      ok = __all_sync(0xffffffffu, gwait(&s.o_full[t], o_n & 1, a.err, abort_s));
+      if (!ok) break;
+      ++o_n;
+      tc_fence_after();
+      // ---- O: to out, or to the workspace and joined by the CTA that is last ----
+      const bool whole = p.n_ctas == 1;
+      const float inv = see > 0 ? 1.0f / l : 0.f;
+      const bool wild = s.wild != 0 && p.tile1 * kTcKeys > see_all;
+      const long long tok_g = p.req.q0 + tok;
+      const int head = p.h * a.group + row % a.group;
+      float* part = a.partial + (paged_slot(blockIdx.x, p.first_cta) * 256 + t * 128 + row) * kLd;
+      T* dst = static_cast<T*>(a.out) + tok_g * a.out_stride + (long long)head * HD;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        float o[32];
+        tc_ld32(o_t + c, o);
+        tc_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) asm volatile("" : "+f"(o[k]));
+        if (!valid) continue;
+        if (l == 0.f) {  // no key of this piece is seen: O may hold 0 * what the others saw
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = 0.f;
+        } else if (wild) {
+#pragma unroll 1
+          for (int k = 0; k < 32; ++k) {
+            const bool pos = s.first[0][c + k] < see, neg = s.first[1][c + k] < see, nan = s.first[2][c + k] < see;
+            float add = 0.f;
+            if (nan || (pos && neg)) add = NAN;
+            else if (pos) add = INFINITY;
+            else if (neg) add = -INFINITY;
+            if (add != 0.f) {
+#pragma unroll
+              for (int q = 0; q < 32; ++q)
+                if (q == k) o[q] += add;
+            }
+          }
+        }
+        if (whole) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            uint4 u;
+            u.x = Frag<T>::pack(o[k] * inv, o[k + 1] * inv);
+            u.y = Frag<T>::pack(o[k + 2] * inv, o[k + 3] * inv);
+            u.z = Frag<T>::pack(o[k + 4] * inv, o[k + 5] * inv);
+            u.w = Frag<T>::pack(o[k + 6] * inv, o[k + 7] * inv);
+            *reinterpret_cast<uint4*>(dst + c + k) = u;
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            *reinterpret_cast<float4*>(part + 4 + c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+        }
+      }
+      if (valid && whole && a.lse)
+        a.lse[tok_g * a.q_heads + head] = see > 0 ? 0.693147180559945309f * (m + log2f(l)) : -INFINITY;
+      if (valid && !whole) *reinterpret_cast<float2*>(part) = make_float2(m, l);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.epi_done[t]);
+      if (!whole) {
+        __threadfence();
+        if (t == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+        else asm volatile("bar.sync 2, 128;" ::: "memory");
+        if ((tid & 127) == 0) {
+          unsigned* ticket = &a.tickets[2 * p.first_cta + t];
+          const bool last = atomicAdd(ticket, 1u) == (unsigned)p.n_ctas - 1;
+          if (last) *ticket = 0u;
+          s.last[t] = last;
+        }
+        if (t == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+        else asm volatile("bar.sync 2, 128;" ::: "memory");
+        if (s.last[t]) {
+          __threadfence();
+          // a warp joins its 32 rows one after the other, HD / 32 columns per lane
+          constexpr int kC = HD / 32;
+          for (int r = 0; r < 32; ++r) {
+            const int rr = (warp & 3) * 32 + r;
+            if (rr >= rows) break;
+            const float* src0 = a.partial + (t * 128 + rr) * (long long)kLd;
+            float mm = -INFINITY;
+            for (int k = 0; k < p.n_ctas; ++k)
+              mm = fmaxf(mm, __ldcg(src0 + paged_slot(p.first_cta + k, p.first_cta) * 256 * kLd));
+            const float b = mm == -INFINITY ? 0.f : mm;
+            float ll = 0.f, acc[kC] = {};
+            for (int k = 0; k < p.n_ctas; ++k) {
+              const float* src = src0 + paged_slot(p.first_cta + k, p.first_cta) * 256 * kLd;
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(src));
+              if (ml.y == 0.f) continue;
+              const float g = paged_exp2(ml.x - b);
+              ll += ml.y * g;
+              if constexpr (kC == 4) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(src + 4 + lane * 4));
+                acc[0] += v.x * g, acc[1] += v.y * g, acc[2] += v.z * g, acc[3] += v.w * g;
+              } else {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(src + 4 + lane * 2));
+                acc[0] += v.x * g, acc[1] += v.y * g;
+              }
+            }
+            const int tk = t0 + t * tile_tokens + rr / a.group, hh = p.h * a.group + rr % a.group;
+            const bool any = p.req.len - p.req.n_new + tk + 1 > 0;
+            const float iv = any ? 1.0f / ll : 0.f;
+            T* out = static_cast<T*>(a.out) + (p.req.q0 + tk) * a.out_stride + (long long)hh * HD + lane * kC;
+            if constexpr (kC == 4)
+              *reinterpret_cast<uint2*>(out) =
+                  make_uint2(Frag<T>::pack(acc[0] * iv, acc[1] * iv), Frag<T>::pack(acc[2] * iv, acc[3] * iv));
+            else
+              *reinterpret_cast<uint32_t*>(out) = Frag<T>::pack(acc[0] * iv, acc[1] * iv);
+            if (a.lse && lane == 0)
+              a.lse[(long long)(p.req.q0 + tk) * a.q_heads + hh] =
+                  any ? 0.693147180559945309f * (mm + log2f(ll)) : -INFINITY;
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTcTmem);
+  }
+}
+
+}  // namespace mcpo
