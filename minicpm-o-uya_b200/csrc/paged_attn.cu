@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kSimtThreads) k_paged_attn_f32(const PagedAttn
   const float* kg = static_cast<const float*>(a.kc);
   const float* vg = static_cast<const float*>(a.vc);
   PagedWalk<kSimtKeys> walk;
-  walk.start(a, &sched, block_tokens, 1);
+  walk.start(a, &sched, block_tokens, 0);
   PagedPiece p;
   while (walk.next(a, &p)) {
     const int t0 = p.b * block_tokens, rows = min(block_tokens, p.req.n_new - t0) * a.group;
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<HD>::kCtas) k_paged_attn_m
   const uint32_t ring_a = smem_addr(ring);
   const int block_tokens = kMmaRows / a.group;
   PagedWalk<kMmaTile> walk;
-  walk.start(a, &sched, block_tokens, 1);
+  walk.start(a, &sched, block_tokens, 0);
   PagedPiece p;
   while (walk.next(a, &p)) {
     const int t0 = p.b * block_tokens, rows = min(block_tokens, p.req.n_new - t0) * a.group;

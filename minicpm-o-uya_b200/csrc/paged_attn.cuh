@@ -6,7 +6,9 @@
 // request, kv head, block, tile, are cut into equal contiguous ranges, one per
 // CTA: ragged lengths leave no CTA with more than one unit above the average,
 // whatever the mix of long and short requests, and the lengths stay on the
-// device.  A block whose tiles lie in several ranges is computed in pieces;
+// device.  A cut within `snap` units of a block's end moves there, since a
+// piece costs as much as a few units.  A block whose tiles lie in several
+// ranges is computed in pieces;
 // each piece leaves its sums in the workspace, and the CTA that finishes last
 // adds them in the ranges' order, so the result does not depend on timing.
 #pragma once
@@ -86,18 +88,65 @@ struct PagedPiece {
 
 template <int KT>
 struct PagedWalk {
-  int block_tokens, ctas;
+  int block_tokens, ctas, snap;
   long long total, u, u1;  // this CTA's next and last unit
   PagedReq req;
   int r, h, b;
   long long block0;  // unit of the block's first tile
 
-  __device__ __forceinline__ long long first_unit(int cta) const { return (long long)cta * total / ctas; }
-  __device__ __forceinline__ int cta_of(long long unit) const { return (int)(((unit + 1) * ctas - 1) / total); }
+  // A cut x inside the block [b0, b0 + n), moved to its start or end when near.
+  __device__ __forceinline__ long long cut(long long x, long long b0, int n) const {
+    const int d = min(snap, n / 2);
+    return x <= b0 + d ? b0 : x >= b0 + n - d ? b0 + n : x;
+  }
+  // The last CTA whose unmoved cut is at or before x.
+  __device__ __forceinline__ int cta_of(long long x) const { return (int)(((x + 1) * ctas - 1) / total); }
+
+  // The request, head and block that hold unit x (x < total).  Block-wide.
+  __device__ __forceinline__ void locate(const PagedAttnArgs& a, PagedShared* s, long long x, long long ex, long long mine,
+                                         int r0, int r1) {
+    __syncthreads();
+    if (x >= ex && x < ex + mine) {  // the thread whose requests hold it finds which
+      long long at = ex;
+      for (int i = r0; i < r1; ++i) {
+        const long long ui = paged_head_units<KT>(paged_req(a, i, block_tokens), block_tokens) * a.kv_heads;
+        if (x < at + ui) {
+          s->r = i;
+          s->before = at;
+          break;
+        }
+        at += ui;
+      }
+    }
+    __syncthreads();
+    r = s->r;
+    req = paged_req(a, r, block_tokens);
+    const long long off = x - s->before, per_head = paged_head_units<KT>(req, block_tokens);
+    h = (int)(off / per_head);
+    b = 0;
+    block0 = s->before + h * per_head;
+    for (int n = paged_tiles<KT>(req, 0, block_tokens); x >= block0 + n; n = paged_tiles<KT>(req, b, block_tokens)) {
+      block0 += n;
+      ++b;
+    }
+  }
+
+  __device__ __forceinline__ void next_block(const PagedAttnArgs& a) {
+    if (++b == req.blocks) {
+      b = 0;
+      if (++h == a.kv_heads) {
+        h = 0;
+        do {
+          req = paged_req(a, ++r, block_tokens);
+        } while (req.blocks == 0);
+      }
+    }
+  }
 
   // Block-wide: every thread of the CTA calls it, and gets the same walk.
-  __device__ __forceinline__ void start(const PagedAttnArgs& a, PagedShared* s, int block_tokens_, int min_units) {
+  __device__ __forceinline__ void start(const PagedAttnArgs& a, PagedShared* s, int block_tokens_, int snap_) {
     block_tokens = block_tokens_;
+    snap = snap_;
     const int n = a.n_req, nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (n + nt - 1) / nt, r0 = min(n, tid * per), r1 = min(n, r0 + per);
     long long mine = 0;
@@ -116,40 +165,29 @@ struct PagedWalk {
       if (w < warp) base += s->red[w];
       all += s->red[w];
     }
-    total = all;
-    ctas = (int)max(1ll, min((long long)gridDim.x, total / min_units));
-    u = blockIdx.x < (unsigned)ctas ? first_unit(blockIdx.x) : total;
-    u1 = blockIdx.x < (unsigned)ctas ? first_unit(blockIdx.x + 1) : total;
-    // the thread whose requests hold unit u walks to the one that has it
     const long long ex = base + incl - mine;
-    if (u < u1 && u >= ex && u < ex + mine) {
-      long long at = ex;
-      for (int i = r0; i < r1; ++i) {
-        const long long ui = paged_head_units<KT>(paged_req(a, i, block_tokens), block_tokens) * a.kv_heads;
-        if (u < at + ui) {
-          s->r = i;
-          s->before = at;
-          break;
-        }
-        at += ui;
-      }
+    total = all;
+    ctas = (int)min((long long)gridDim.x, total);
+    u = u1 = total;
+    if ((int)blockIdx.x >= ctas) return;  // the same for the whole block
+    const long long x0 = (long long)blockIdx.x * total / ctas, x1 = (long long)(blockIdx.x + 1) * total / ctas;
+    if (x1 < total) {
+      locate(a, s, x1, ex, mine, r0, r1);
+      u1 = cut(x1, block0, paged_tiles<KT>(req, b, block_tokens));
     }
-    __syncthreads();
-    if (u < u1) {
-      r = s->r;
-      req = paged_req(a, r, block_tokens);
-      const long long off = u - s->before, per_head = paged_head_units<KT>(req, block_tokens);
-      h = (int)(off / per_head);
-      b = 0;
-      block0 = s->before + h * per_head;
-      while (u >= block0 + paged_tiles<KT>(req, b, block_tokens)) block0 += paged_tiles<KT>(req, b++, block_tokens);
+    locate(a, s, x0, ex, mine, r0, r1);
+    const int len = paged_tiles<KT>(req, b, block_tokens);
+    u = cut(x0, block0, len);
+    if (u < u1 && u == block0 + len) {
+      block0 = u;
+      next_block(a);
     }
   }
 
   // The next piece of this CTA's range; false at its end.
   __device__ __forceinline__ bool next(const PagedAttnArgs& a, PagedPiece* p) {
     if (u >= u1) return false;
-    const int n = paged_tiles<KT>(req, b, block_tokens);
+    const int n = paged_tiles<KT>(req, b, block_tokens), d = min(snap, n / 2);
     p->req = req;
     p->r = r;
     p->h = h;
@@ -157,20 +195,14 @@ struct PagedWalk {
     p->n_tiles = n;
     p->tile0 = (int)(u - block0);
     p->tile1 = (int)min((long long)n, u1 - block0);
-    p->first_cta = cta_of(block0);
-    p->n_ctas = cta_of(block0 + n - 1) - p->first_cta + 1;
+    // the CTAs whose moved ranges meet the block: from the last cut that is at
+    // or moves to its start, to the last one before those that move to its end
+    p->first_cta = cta_of(block0 + d);
+    p->n_ctas = max(0, cta_of(block0 + n - d - 1) - p->first_cta) + 1;
     u = block0 + p->tile1;
     if (p->tile1 == n && u < u1) {
       block0 = u;
-      if (++b == req.blocks) {
-        b = 0;
-        if (++h == a.kv_heads) {
-          h = 0;
-          do {
-            req = paged_req(a, ++r, block_tokens);
-          } while (req.blocks == 0);
-        }
-      }
+      next_block(a);
     }
     return true;
   }

@@ -7,7 +7,8 @@
 // 16-bit values, and O += P V reads them from there.  Roles: warps 0-3 and 4-7
 // are the softmax of tile 0 and 1, warp 8 issues the MMAs, warp 9 the TMA
 // loads of Q and of K and V pages (a ring of 128-key stages that both tiles
-// read).  The MMAs are issued P V (0), Q K^T (0), P V (1), Q K^T (1), ...: while
+// read); warps 10 and 11 only fill the warpgroup, whose registers go to the
+// softmax warps.  The MMAs are issued P V (0), Q K^T (0), P V (1), Q K^T (1), ...: while
 // one tile's softmax runs, the tensor cores have the other tile's products.
 //
 // Rows keep the maximum they began with until a score exceeds it by 2^8;
@@ -24,7 +25,7 @@
 
 namespace mcpo {
 
-constexpr int kTcRows = 128, kTcKeys = 128, kTcThreads = 320;
+constexpr int kTcRows = 128, kTcKeys = 128, kTcThreads = 384;
 constexpr int kTcMaxCtas = 240;  // by the workspace
 constexpr uint32_t kTcTmem = 512;
 
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __shared__ PagedPiece pieces[kTcThreads / 32];
   {
     PagedWalk<kTcKeys> walk;
-    walk.start(a, &sched, block_tokens, 1);  // has barriers: the inits above are seen behind them
+    walk.start(a, &sched, block_tokens, 2);  // has barriers: the inits above are seen behind them
     if (lane == 0) walks[warp] = walk;
   }
   tc_fence_before();
@@ -203,7 +204,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     return __shfl_sync(0xffffffffu, (int)more, 0) != 0;
   };
 
-  if (warp == 9) {
+  // 384 threads start with 168 registers each (64512): 208 * 256 + 80 * 128 = 63488
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 9) {
     // ---- loads: one lane per box (a page's rows x 64 values) ----
     const int box_rows = min(1 << a.page_shift, kTcKeys);
     const int page_of = lane / kHalves, half = lane % kHalves;  // this lane's box of a stage
@@ -257,7 +261,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_wait(&s.kv_full[i % kStages], (i / kStages) & 1, a.err);
     }
     __syncwarp();
-  } else if (warp == 8) {
+    } else if (warp == 8) {
     // ---- MMAs ----
     if (lane == 0) {
       constexpr uint32_t kType = sizeof(T) == 2 && Frag<T>::kExp == 0x7f807f80u ? 1u : 0u;  // 1: bf16
@@ -326,7 +330,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     }
     __syncwarp();
+    }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax of tile t: thread = row ----
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -521,44 +527,71 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         else asm volatile("bar.sync 2, 128;" ::: "memory");
         if (s.last[t]) {
           __threadfence();
-          // a warp joins its 32 rows one after the other, HD / 32 columns per lane
+          // A warp joins its 32 rows, 16 at a time: lane r has row r's
+          // statistics, and all lanes HD / 32 columns of every row, so that 16
+          // loads are in flight for each piece.
           constexpr int kC = HD / 32;
-          for (int r = 0; r < 32; ++r) {
-            const int rr = (warp & 3) * 32 + r;
-            if (rr >= rows) break;
-            const float* src0 = a.partial + (t * 128 + rr) * (long long)kLd;
-            float mm = -INFINITY;
+          const int w0 = (warp & 3) * 32;
+          const float* src0 = a.partial + (long long)(t * 128 + w0) * kLd;
+          const long long slot_f = 256ll * kLd;
+          float mm = -INFINITY, ll = 0.f;
+          if (valid)
             for (int k = 0; k < p.n_ctas; ++k)
-              mm = fmaxf(mm, __ldcg(src0 + paged_slot(p.first_cta + k, p.first_cta) * 256 * kLd));
-            const float b = mm == -INFINITY ? 0.f : mm;
-            float ll = 0.f, acc[kC] = {};
+              mm = fmaxf(mm, __ldcg(src0 + paged_slot(p.first_cta + k, p.first_cta) * slot_f + lane * kLd));
+          const float b = mm == -INFINITY ? 0.f : mm;
+#pragma unroll 1
+          for (int r0 = 0; r0 < 32; r0 += 16) {
+            float acc[16][kC];
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+#pragma unroll
+              for (int c = 0; c < kC; ++c) acc[r][c] = 0.f;
+            ll = 0.f;
+#pragma unroll 1
             for (int k = 0; k < p.n_ctas; ++k) {
-              const float* src = src0 + paged_slot(p.first_cta + k, p.first_cta) * 256 * kLd;
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(src));
-              if (ml.y == 0.f) continue;
-              const float g = paged_exp2(ml.x - b);
+              const float* src = src0 + paged_slot(p.first_cta + k, p.first_cta) * slot_f;
+              float4 v[16];
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (w0 + r0 + r < rows) {
+                  const float* at = src + (r0 + r) * kLd + 4 + lane * kC;
+                  if constexpr (kC == 4) {
+                    v[r] = __ldcg(reinterpret_cast<const float4*>(at));
+                  } else {
+                    const float2 h = __ldcg(reinterpret_cast<const float2*>(at));
+                    v[r].x = h.x, v[r].y = h.y;
+                  }
+                }
+              }
+              float2 ml = make_float2(-INFINITY, 0.f);
+              if (valid) ml = __ldcg(reinterpret_cast<const float2*>(src + lane * kLd));
+              const float g = ml.y == 0.f ? 0.f : paged_exp2(ml.x - b);
               ll += ml.y * g;
-              if constexpr (kC == 4) {
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(src + 4 + lane * 4));
-                acc[0] += v.x * g, acc[1] += v.y * g, acc[2] += v.z * g, acc[3] += v.w * g;
-              } else {
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(src + 4 + lane * 2));
-                acc[0] += v.x * g, acc[1] += v.y * g;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const float gr = __shfl_sync(0xffffffffu, g, r0 + r);
+                acc[r][0] += v[r].x * gr, acc[r][1] += v[r].y * gr;
+                if constexpr (kC == 4) acc[r][2] += v[r].z * gr, acc[r][3] += v[r].w * gr;
               }
             }
-            const int tk = t0 + t * tile_tokens + rr / a.group, hh = p.h * a.group + rr % a.group;
-            const bool any = p.req.len - p.req.n_new + tk + 1 > 0;
-            const float iv = any ? 1.0f / ll : 0.f;
-            T* out = static_cast<T*>(a.out) + (p.req.q0 + tk) * a.out_stride + (long long)hh * HD + lane * kC;
-            if constexpr (kC == 4)
-              *reinterpret_cast<uint2*>(out) =
-                  make_uint2(Frag<T>::pack(acc[0] * iv, acc[1] * iv), Frag<T>::pack(acc[2] * iv, acc[3] * iv));
-            else
-              *reinterpret_cast<uint32_t*>(out) = Frag<T>::pack(acc[0] * iv, acc[1] * iv);
-            if (a.lse && lane == 0)
-              a.lse[(long long)(p.req.q0 + tk) * a.q_heads + hh] =
-                  any ? 0.693147180559945309f * (mm + log2f(ll)) : -INFINITY;
+            const float iv = see > 0 ? 1.0f / ll : 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int rr = w0 + r0 + r;
+              const float ir = __shfl_sync(0xffffffffu, iv, r0 + r);
+              if (rr >= rows) continue;
+              T* out = static_cast<T*>(a.out) + (p.req.q0 + t0 + t * tile_tokens + rr / a.group) * a.out_stride +
+                       (long long)(p.h * a.group + rr % a.group) * HD + lane * kC;
+              if constexpr (kC == 4)
+                *reinterpret_cast<uint2*>(out) = make_uint2(Frag<T>::pack(acc[r][0] * ir, acc[r][1] * ir),
+                                                            Frag<T>::pack(acc[r][2] * ir, acc[r][3] * ir));
+              else
+                *reinterpret_cast<uint32_t*>(out) = Frag<T>::pack(acc[r][0] * ir, acc[r][1] * ir);
+            }
           }
+          if (valid && a.lse)
+            a.lse[tok_g * a.q_heads + head] = see > 0 ? 0.693147180559945309f * (mm + log2f(ll)) : -INFINITY;
         }
       }
     }
