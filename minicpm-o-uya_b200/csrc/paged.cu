@@ -443,8 +443,7 @@ int minicpmo_gpu_paged_plan(const int32_t* lens, const int32_t* new_lens, size_t
     return paged_error(error, error_cap, "error: %s: token capacity %zu", op, token_capacity);
   if (cu_new == lens || cu_new == new_lens || lens_out == new_lens)
     return paged_error(error, error_cap, "error: %s: only lens_out and ring_state_out may be inputs' buffers", op);
-  if (!paged_on_device(lens, op, error, error_cap) || !paged_on_device(slots ? (const void*)slots : status, op, error, error_cap))
-    return 0;
+  if (!paged_on_device(lens, op, error, error_cap)) return 0;
   PlanArgs a{};
   a.lens = lens;
   a.new_lens = new_lens;
@@ -465,9 +464,10 @@ int minicpmo_gpu_paged_plan(const int32_t* lens, const int32_t* new_lens, size_t
   a.status = status;
   const size_t smem = (4 * n_req + 3) * sizeof(int);
   static_assert((4 * MINICPMO_PAGED_MAX_REQUESTS + 3) * sizeof(int) <= 160 * 1024, "plan prefix sums fit shared memory");
-  cudaError_t e = cudaSuccess;
-  if (smem > 46 * 1024)
-    e = cudaFuncSetAttribute(k_paged_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  static OncePerDevice once;
+  cudaError_t e = once([] {
+    return cudaFuncSetAttribute(k_paged_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  });
   if (e == cudaSuccess) {
     // one CTA does a decode step; a cluster where tokens or requests give each CTA a turn of work
     const size_t most = token_capacity > n_req ? token_capacity : n_req;
@@ -516,7 +516,7 @@ int minicpmo_gpu_paged_append(const minicpmo_paged_cache* cache, const void* q, 
       !aligned16(rope_sin) || (q_norm && !aligned16(q_norm)) || (k_norm && !aligned16(k_norm)) ||
       (q_heads && (!aligned16(q) || !aligned16(q_out) || q_stride * isz % 16 || q_out_stride * csz % 16)))
     return paged_error(error, error_cap, "error: %s: pointers and strides must be multiples of 16 bytes", op);
-  if (!paged_on_device(cache->k, op, error, error_cap) || !paged_on_device(k, op, error, error_cap)) return 0;
+  if (!paged_on_device(cache->k, op, error, error_cap)) return 0;
   AppendArgs a{};
   a.q = q;
   a.k = k;

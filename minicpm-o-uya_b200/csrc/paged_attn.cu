@@ -558,23 +558,28 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<HD>::kCtas) k_paged_attn_m
   }
 }
 
-template <typename K>
-cudaError_t big_smem(K kernel, size_t bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
-
-cudaError_t sm_count(int* n) {
+// The kernel's shared memory and the SM count, set up once per device.
+template <auto kKernel>
+cudaError_t ready(size_t smem, int* sms) {
+  static OncePerDevice once;
+  static int count[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64) return cudaErrorInvalidDevice;
+  e = once([&] {
+    cudaError_t r = cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev);
+    if (r == cudaSuccess) r = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    return r;
+  });
+  *sms = count[dev];
   return e;
 }
 
 template <int HD>
 cudaError_t launch_f32(const PagedAttnArgs& a, cudaStream_t st) {
   int sms = 0;
-  cudaError_t e = sm_count(&sms);
-  if (e == cudaSuccess) e = big_smem(k_paged_attn_f32<HD>, sizeof(SimtSmem<HD>));
+  const cudaError_t e = ready<k_paged_attn_f32<HD>>(sizeof(SimtSmem<HD>), &sms);
   if (e != cudaSuccess) return e;
   const int ctas = HD == 256 ? sms : 2 * sms;  // residents by shared memory
   k_paged_attn_f32<HD><<<ctas < kPagedMaxCtas ? ctas : kPagedMaxCtas, kSimtThreads, sizeof(SimtSmem<HD>), st>>>(a);
@@ -586,8 +591,7 @@ cudaError_t launch_mma(const PagedAttnArgs& a, cudaStream_t st) {
   using Cfg = MmaCfg<HD>;
   static_assert(Cfg::kSmem >= kMmaWarps * kMmaRows * (HD + 4) * 4, "the joined sums fit the rings");
   int sms = 0;
-  cudaError_t e = sm_count(&sms);
-  if (e == cudaSuccess) e = big_smem(k_paged_attn_mma<T, HD>, Cfg::kSmem);
+  const cudaError_t e = ready<k_paged_attn_mma<T, HD>>(Cfg::kSmem, &sms);
   if (e != cudaSuccess) return e;
   const int ctas = Cfg::kCtas * sms;
   k_paged_attn_mma<T, HD><<<ctas < kPagedMaxCtas ? ctas : kPagedMaxCtas, kMmaThreads, Cfg::kSmem, st>>>(a);
@@ -646,8 +650,7 @@ bool tc_maps(TcMaps* m, const PagedAttnArgs& a, int hd, bool bf16) {
 template <typename T, int HD>
 cudaError_t launch_tc(const PagedAttnArgs& a, const TcMaps& m, cudaStream_t st) {
   int sms = 0;
-  cudaError_t e = sm_count(&sms);
-  if (e == cudaSuccess) e = big_smem(k_paged_attn_tc<T, HD>, TcCfg<HD>::kSmem);
+  const cudaError_t e = ready<k_paged_attn_tc<T, HD>>(TcCfg<HD>::kSmem, &sms);
   if (e != cudaSuccess) return e;
   k_paged_attn_tc<T, HD><<<sms < kTcMaxCtas ? sms : kTcMaxCtas, kTcThreads, TcCfg<HD>::kSmem, st>>>(a, m);
   return cudaGetLastError();
@@ -704,7 +707,7 @@ extern "C" int minicpmo_gpu_paged_attention(const minicpmo_paged_cache* cache, c
     return paged_error(error, error_cap,
                        "error: %s: pointers and strides must be multiples of 16 bytes, the workspace of 256", op);
   if (!(scale > -INFINITY && scale < INFINITY)) return paged_error(error, error_cap, "error: %s: scale is not finite", op);
-  if (!paged_on_device(cache->k, op, error, error_cap) || !paged_on_device(workspace, op, error, error_cap)) return 0;
+  if (!paged_on_device(cache->k, op, error, error_cap)) return 0;
   PagedAttnArgs a{};
   a.q = q;
   a.out = out;

@@ -637,9 +637,13 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
 template <typename T>
 cudaError_t launch_sample(const SampleArgs& a, int cluster, cudaStream_t st) {
   const size_t smem = sizeof(Shared) + (size_t)a.slice * 4;
-  cudaError_t e = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)(sizeof(Shared) + (size_t)kSmpSlice * 4));
-  if (e == cudaSuccess && cluster > 8) e = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  static OncePerDevice once;
+  cudaError_t e = once([] {
+    cudaError_t r = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)(sizeof(Shared) + (size_t)kSmpSlice * 4));
+    if (r == cudaSuccess) r = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    return r;
+  });
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * cluster));
@@ -678,7 +682,7 @@ extern "C" int minicpmo_gpu_sample(const void* logits, int dtype, size_t rows, s
   if (stride < vocab || stride > (1ull << 40))
     return paged_error(error, error_cap, "error: %s: rows of %zu tokens, %zu apart", op, vocab, stride);
   if (reinterpret_cast<uintptr_t>(logits) % esz) return paged_error(error, error_cap, "error: %s: misaligned logits", op);
-  if (!paged_on_device(logits, op, error, error_cap) || !paged_on_device(tokens, op, error, error_cap)) return 0;
+  if (!paged_on_device(logits, op, error, error_cap)) return 0;
   SampleArgs a{};
   a.logits = logits;
   a.stride = (long long)stride;

@@ -15,6 +15,7 @@ be captured into a CUDA graph (with all outputs given).  ``include/minicpmo_gpu.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from typing import NamedTuple, Optional
 
 import torch
@@ -26,6 +27,8 @@ WORKSPACE_BYTES = 64 << 20  # MINICPMO_PAGED_WORKSPACE_BYTES
 MAX_REQUESTS = 8192  # MINICPMO_PAGED_MAX_REQUESTS
 
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+_local = threading.local()  # this thread's error buffer
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -33,53 +36,66 @@ def _check(cond: bool, msg: str) -> None:
         raise GpuError("error: " + msg)
 
 
-def _call(fn, device: torch.device, *args) -> None:
-    err = C.create_string_buffer(ERR_CAP)
-    if torch.cuda.current_device() == device.index:
-        ok = fn(*args, torch.cuda.current_stream(device).cuda_stream, err, ERR_CAP)
+def _call(name: str, index: int, *args) -> None:
+    """The library's entry point with the device current and its current stream, the message raised on refusal."""
+    try:
+        err = _local.err
+    except AttributeError:
+        err = _local.err = C.create_string_buffer(ERR_CAP)
+    fn = getattr(lib(), name)
+    if torch._C._cuda_getDevice() == index:
+        ok = fn(*args, torch._C._cuda_getCurrentRawStream(index), err, ERR_CAP)
     else:
-        with torch.cuda.device(device):
-            ok = fn(*args, torch.cuda.current_stream(device).cuda_stream, err, ERR_CAP)
+        with torch.cuda.device(index):
+            ok = fn(*args, torch._C._cuda_getCurrentRawStream(index), err, ERR_CAP)
     if not ok:
         raise GpuError(err.value.decode())
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _tensor(op: str, name: str, t: torch.Tensor, device: torch.device, dtype, shape) -> None:
-    """t: a contiguous tensor of that type and shape on `device`."""
-    if t.dtype != dtype or t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise GpuError(f"error: {op}: {name} must be a contiguous {dtype} tensor {tuple(shape)} on {device}, got "
+def _tensor(op: str, name: str, t: torch.Tensor, index: int, dtype, shape) -> int:
+    """The address of t, a contiguous tensor of that type and shape on device `index`."""
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape or not t.is_contiguous():
+        raise GpuError(f"error: {op}: {name} must be a contiguous {dtype} tensor {tuple(shape)} on cuda:{index}, got "
                        f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
-def _rows(op: str, name: str, t: torch.Tensor, device: torch.device, hd: int) -> int:
+def _rows(op: str, name: str, t: torch.Tensor, index: int, hd: int) -> int:
     """t: [tokens, heads, hd] with contiguous heads; the elements between two tokens."""
-    st = t.stride()
-    if t.dim() != 3 or t.device != device or t.shape[2] != hd or st[2] != 1 or (st[1] != hd and t.shape[1] > 1):
-        raise GpuError(f"error: {op}: {name} must be [tokens, heads, {hd}] on {device} with contiguous heads, got "
-                       f"{tuple(t.shape)} with strides {tuple(st)} on {t.device}")
+    st, shape = t.stride(), t.shape
+    if len(shape) != 3 or t.get_device() != index or shape[2] != hd or st[2] != 1 or (st[1] != hd and shape[1] > 1):
+        raise GpuError(f"error: {op}: {name} must be [tokens, heads, {hd}] on cuda:{index} with contiguous heads, got "
+                       f"{tuple(shape)} with strides {tuple(st)} on {t.device}")
     # the stride of a single token says nothing, and may be anything
-    return st[0] if t.shape[0] > 1 else max(st[0], t.shape[1] * hd)
+    return st[0] if shape[0] > 1 else max(st[0], shape[1] * hd)
 
 
 def _cache(op: str, k: torch.Tensor, v: torch.Tensor) -> PagedCache:
     """The C description of one layer's K and V pages, [pages, page_size, kv_heads, head_dim] views of any layout."""
-    if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.device != v.device:
+    shape, st = k.shape, k.stride()
+    if len(shape) != 4 or shape != v.shape or st != v.stride() or k.dtype is not v.dtype or k.get_device() != v.get_device():
         raise GpuError(f"error: {op}: k_cache and v_cache must be [pages, page_size, kv_heads, head_dim] tensors alike")
-    if not k.is_cuda or k.dtype not in _DTYPES or k.stride(3) != 1:
+    dtype = _DTYPES.get(k.dtype)
+    if k.get_device() < 0 or dtype is None or st[3] != 1:
         raise GpuError(f"error: {op}: caches must be f32, f16 or bf16 CUDA tensors with contiguous rows, got {k.dtype} "
                        f"on {k.device}")
-    n, ps, kv, hd = k.shape
-    sp, st, sh, _ = k.stride()
+    n, ps, kv, hd = shape
+    sp, st, sh, _ = st
     # a dimension of one has no stride of its own: take the contiguous one
     if kv == 1:
         sh = hd
     if n == 1:
         sp = max(st * ps, sh * kv)
-    return PagedCache(k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], ps, kv, hd, n, sp, st, sh)
+    return PagedCache(k.data_ptr(), v.data_ptr(), dtype, ps, kv, hd, n, sp, st, sh)
+
+
+def _table(op: str, t: torch.Tensor, n: int, index: int) -> int:
+    """The entries between two rows of a block table [n, max_pages]."""
+    shape, st = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != n or t.dtype is not _I32 or t.get_device() != index or st[1] != 1:
+        raise GpuError(f"error: {op}: block_table must be an int32 tensor [{n}, max_pages] on cuda:{index} with "
+                       f"contiguous rows")
+    return st[0] if n > 1 else shape[1]
 
 
 class PagedPlan(NamedTuple):
@@ -102,34 +118,25 @@ def plan(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, 
     inputs themselves.  A step that does not fit (see status) changes nothing and plans no token.
     """
     op = "paged plan"
-    dev, n = lens.device, lens.shape[0] if lens.dim() == 1 else 0
-    _check(lens.is_cuda and n > 0, f"{op}: lens must be a CUDA tensor [requests]")
-    i32, i64 = torch.int32, torch.int64
-    _tensor(op, "lens", lens, dev, i32, (n,))
-    _tensor(op, "new_lens", new_lens, dev, i32, (n,))
-    _tensor(op, "ring_state", ring_state, dev, i64, (2,))
-    _check(free_ring.dim() == 1, f"{op}: free_ring must be [capacity]")
-    _tensor(op, "free_ring", free_ring, dev, i32, free_ring.shape)
-    if (block_table.dim() != 2 or block_table.shape[0] != n or block_table.dtype != i32 or block_table.device != dev
-            or block_table.stride(1) != 1):
-        raise GpuError(f"error: {op}: block_table must be an int32 tensor [{n}, max_pages] on {dev} with contiguous rows")
+    dev, n = lens.get_device(), lens.numel()
+    _check(dev >= 0 and n > 0, f"{op}: lens must be a CUDA tensor [requests]")
     _check(token_capacity >= 0 and page_size > 0, f"{op}: token_capacity {token_capacity}, page_size {page_size}")
+    stride, ring = _table(op, block_table, n, dev), free_ring.numel()
+    inputs = (_tensor(op, "lens", lens, dev, _I32, (n,)), _tensor(op, "new_lens", new_lens, dev, _I32, (n,)), n,
+              block_table.data_ptr(), block_table.shape[1], stride, _tensor(op, "free_ring", free_ring, dev, _I32, (ring,)),
+              ring, _tensor(op, "ring_state", ring_state, dev, _I64, (2,)), page_size, token_capacity)
     if out is None:
-        with torch.cuda.device(dev):
-            out = PagedPlan(torch.empty_like(lens), torch.empty_like(ring_state), lens.new_empty(n + 1),
-                            lens.new_empty(token_capacity), ring_state.new_empty(token_capacity), lens.new_empty(2))
+        a, b, c, d = lens.new_empty(2 * n + 3 + token_capacity).split((n, n + 1, token_capacity, 2))
+        e, f = ring_state.new_empty(2 + token_capacity).split((2, token_capacity))
+        out = PagedPlan(a, e, b, c, f, d)
     else:
-        _tensor(op, "out.lens", out.lens, dev, i32, (n,))
-        _tensor(op, "out.ring_state", out.ring_state, dev, i64, (2,))
-        _tensor(op, "out.cu_new", out.cu_new, dev, i32, (n + 1,))
-        _tensor(op, "out.positions", out.positions, dev, i32, (token_capacity,))
-        _tensor(op, "out.slots", out.slots, dev, i64, (token_capacity,))
-        _tensor(op, "out.status", out.status, dev, i32, (2,))
-    max_pages = block_table.shape[1]
-    _call(lib().minicpmo_gpu_paged_plan, dev, lens.data_ptr(), new_lens.data_ptr(), n, block_table.data_ptr(), max_pages,
-          block_table.stride(0) if n > 1 else max_pages, free_ring.data_ptr(), free_ring.shape[0], ring_state.data_ptr(),
-          page_size, token_capacity, out.lens.data_ptr(), out.ring_state.data_ptr(), out.cu_new.data_ptr(),
-          out.positions.data_ptr(), out.slots.data_ptr(), out.status.data_ptr())
+        _tensor(op, "out.lens", out.lens, dev, _I32, (n,))
+        _tensor(op, "out.ring_state", out.ring_state, dev, _I64, (2,))
+        _tensor(op, "out.cu_new", out.cu_new, dev, _I32, (n + 1,))
+        _tensor(op, "out.positions", out.positions, dev, _I32, (token_capacity,))
+        _tensor(op, "out.slots", out.slots, dev, _I64, (token_capacity,))
+        _tensor(op, "out.status", out.status, dev, _I32, (2,))
+    _call("minicpmo_gpu_paged_plan", dev, *inputs, *(t.data_ptr() for t in out))
     return out
 
 
@@ -147,33 +154,34 @@ def append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     """
     op = "paged append"
     cache = _cache(op, k_cache, v_cache)
-    dev, hd, n = k_cache.device, k_cache.shape[3], k.shape[0]
+    dev, hd, n, ctype = k_cache.get_device(), k_cache.shape[3], k.shape[0], k_cache.dtype
     ks, vs = _rows(op, "k", k, dev, hd), _rows(op, "v", v, dev, hd)
-    _check(k.dtype in _DTYPES and v.dtype == k.dtype and k.shape == v.shape and k.shape[1] == k_cache.shape[2],
-           f"{op}: k and v must be alike, with the cache's {k_cache.shape[2]} heads")
-    _tensor(op, "positions", positions, dev, torch.int32, (n,))
-    _tensor(op, "slots", slots, dev, torch.int64, (n,))
+    dtype = _DTYPES.get(k.dtype)
+    if dtype is None or v.dtype is not k.dtype or k.shape != v.shape or k.shape[1] != k_cache.shape[2]:
+        raise GpuError(f"error: {op}: k and v must be alike, with the cache's {k_cache.shape[2]} heads")
     _check(rope_cos.dim() == 2, f"{op}: rope tables must be [context, head_dim / 2]")
-    _tensor(op, "rope_cos", rope_cos, dev, torch.float32, (rope_cos.shape[0], hd // 2))
-    _tensor(op, "rope_sin", rope_sin, dev, torch.float32, rope_cos.shape)
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w is not None:
-            _tensor(op, name, w, dev, torch.float32, (hd,))
+    context = rope_cos.shape[0]
     heads = qs = os = 0
     if q is not None:
         heads, qs = q.shape[1], _rows(op, "q", q, dev, hd)
-        _check(q.dtype == k.dtype and q.shape[0] == n, f"{op}: q must have k's type and tokens")
+        if q.dtype is not k.dtype or q.shape[0] != n:
+            raise GpuError(f"error: {op}: q must have k's type and tokens")
         if q_out is None:
-            q_out = torch.zeros(n, heads, hd, dtype=k_cache.dtype, device=dev)
+            q_out = torch.zeros(n, heads, hd, dtype=ctype, device=k_cache.device)
         os = _rows(op, "q_out", q_out, dev, hd)
-        _check(q_out.dtype == k_cache.dtype and q_out.shape == q.shape, f"{op}: q_out must have the cache's type and q's shape")
+        if q_out.dtype is not ctype or q_out.shape != q.shape:
+            raise GpuError(f"error: {op}: q_out must have the cache's type and q's shape")
     else:
         _check(q_out is None, f"{op}: q_out without q")
-    if status is not None:
-        _tensor(op, "status", status, dev, torch.int32, (1,))
-    _call(lib().minicpmo_gpu_paged_append, dev, C.byref(cache), _ptr(q), k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], n,
-          heads, qs, ks, vs, _ptr(q_norm), _ptr(k_norm), eps, rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0],
-          positions.data_ptr(), slots.data_ptr(), _ptr(q_out), os, _ptr(status))
+    _call("minicpmo_gpu_paged_append", dev, C.byref(cache), None if q is None else q.data_ptr(), k.data_ptr(),
+          v.data_ptr(), dtype, n, heads, qs, ks, vs,
+          None if q_norm is None else _tensor(op, "q_norm", q_norm, dev, _F32, (hd,)),
+          None if k_norm is None else _tensor(op, "k_norm", k_norm, dev, _F32, (hd,)), eps,
+          _tensor(op, "rope_cos", rope_cos, dev, _F32, (context, hd // 2)),
+          _tensor(op, "rope_sin", rope_sin, dev, _F32, (context, hd // 2)), context,
+          _tensor(op, "positions", positions, dev, _I32, (n,)), _tensor(op, "slots", slots, dev, _I64, (n,)),
+          None if q_out is None else q_out.data_ptr(), os,
+          None if status is None else _tensor(op, "status", status, dev, _I32, (1,)))
     return q_out
 
 
@@ -194,28 +202,22 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blo
     """
     op = "paged attention"
     cache = _cache(op, k_cache, v_cache)
-    dev, hd, n = k_cache.device, k_cache.shape[3], lens.shape[0]
-    qs = _rows(op, "q", q, dev, hd)
-    _check(q.dtype == k_cache.dtype, f"{op}: q must have the cache's type {k_cache.dtype}, got {q.dtype}")
-    _tensor(op, "lens", lens, dev, torch.int32, (n,))
-    _tensor(op, "cu_new", cu_new, dev, torch.int32, (n + 1,))
-    if (block_table.dim() != 2 or block_table.shape[0] != n or block_table.dtype != torch.int32
-            or block_table.device != dev or block_table.stride(1) != 1):
-        raise GpuError(f"error: {op}: block_table must be an int32 tensor [{n}, max_pages] on {dev} with contiguous rows")
-    _check(workspace.device == dev and workspace.is_contiguous()
-           and workspace.numel() * workspace.element_size() >= WORKSPACE_BYTES,
-           f"{op}: the workspace must be {WORKSPACE_BYTES} contiguous bytes on {dev}")
+    dev, hd, n = k_cache.get_device(), k_cache.shape[3], lens.numel()
+    qs, stride = _rows(op, "q", q, dev, hd), _table(op, block_table, n, dev)
+    if q.dtype is not k_cache.dtype:
+        raise GpuError(f"error: {op}: q must have the cache's type {k_cache.dtype}, got {q.dtype}")
+    if workspace.get_device() != dev or not workspace.is_contiguous() or workspace.nbytes < WORKSPACE_BYTES:
+        raise GpuError(f"error: {op}: the workspace must be {WORKSPACE_BYTES} contiguous bytes on cuda:{dev}")
     if out is None:
-        out = torch.zeros(q.shape, dtype=q.dtype, device=dev)
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
     os = _rows(op, "out", out, dev, hd)
-    _check(out.dtype == q.dtype and out.shape == q.shape, f"{op}: out must have q's type and shape")
-    if lse is not None:
-        _tensor(op, "lse", lse, dev, torch.float32, q.shape[:2])
-    max_pages = block_table.shape[1]
-    _call(lib().minicpmo_gpu_paged_attention, dev, C.byref(cache), q.data_ptr(), q.shape[0], q.shape[1], qs,
-          block_table.data_ptr(), max_pages, block_table.stride(0) if n > 1 else max_pages, lens.data_ptr(),
-          cu_new.data_ptr(), n, hd ** -0.5 if scale is None else scale, out.data_ptr(), os, _ptr(lse),
-          workspace.data_ptr())
+    if out.dtype is not q.dtype or out.shape != q.shape:
+        raise GpuError(f"error: {op}: out must have q's type and shape")
+    tokens, heads, _ = q.shape
+    _call("minicpmo_gpu_paged_attention", dev, C.byref(cache), q.data_ptr(), tokens, heads, qs, block_table.data_ptr(),
+          block_table.shape[1], stride, _tensor(op, "lens", lens, dev, _I32, (n,)),
+          _tensor(op, "cu_new", cu_new, dev, _I32, (n + 1,)), n, hd ** -0.5 if scale is None else scale, out.data_ptr(),
+          os, None if lse is None else _tensor(op, "lse", lse, dev, _F32, (tokens, heads)), workspace.data_ptr())
     return out
 
 
@@ -231,23 +233,19 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: Optional[to
     """One token per row of logits [rows, vocab] (f32, f16 or bf16) from uniform random numbers f32 [rows]
     (``minicpmo_gpu_sample``): temperature, top_p, min_p f32 [rows] and top_k int32 [rows], each None for off."""
     op = "sample"
-    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in _DTYPES or logits.stride(1) != 1:
+    shape, dev, dtype = logits.shape, logits.get_device(), _DTYPES.get(logits.dtype)
+    if dev < 0 or len(shape) != 2 or dtype is None or logits.stride(1) != 1:
         raise GpuError(f"error: {op}: logits must be a [rows, vocab] f32, f16 or bf16 CUDA tensor with contiguous rows")
-    dev, (n, vocab) = logits.device, logits.shape
-    f32 = torch.float32
-    _tensor(op, "uniform", uniform, dev, f32, (n,))
-    for name, t, dtype in (("temperature", temperature, f32), ("top_k", top_k, torch.int32), ("top_p", top_p, f32),
-                           ("min_p", min_p, f32)):
-        if t is not None:
-            _tensor(op, name, t, dev, dtype, (n,))
+    n, vocab = shape
+    rows = (n,)
     if out is None:
-        words = torch.empty(3, n, dtype=torch.int32, device=dev)
-        out = Sampled(words[0], words[1].view(f32), words[2])
-    else:
-        _tensor(op, "out.token", out.token, dev, torch.int32, (n,))
-        _tensor(op, "out.prob", out.prob, dev, f32, (n,))
-        _tensor(op, "out.kept", out.kept, dev, torch.int32, (n,))
-    _call(lib().minicpmo_gpu_sample, dev, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab,
-          logits.stride(0) if n > 1 else vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
-          uniform.data_ptr(), out.token.data_ptr(), out.prob.data_ptr(), out.kept.data_ptr())
+        token, prob, kept = torch.empty(3, n, dtype=_I32, device=logits.device).unbind()
+        out = Sampled(token, prob.view(_F32), kept)
+    _call("minicpmo_gpu_sample", dev, logits.data_ptr(), dtype, n, vocab, logits.stride(0) if n > 1 else vocab,
+          None if temperature is None else _tensor(op, "temperature", temperature, dev, _F32, rows),
+          None if top_k is None else _tensor(op, "top_k", top_k, dev, _I32, rows),
+          None if top_p is None else _tensor(op, "top_p", top_p, dev, _F32, rows),
+          None if min_p is None else _tensor(op, "min_p", min_p, dev, _F32, rows),
+          _tensor(op, "uniform", uniform, dev, _F32, rows), _tensor(op, "out.token", out.token, dev, _I32, rows),
+          _tensor(op, "out.prob", out.prob, dev, _F32, rows), _tensor(op, "out.kept", out.kept, dev, _I32, rows))
     return out
