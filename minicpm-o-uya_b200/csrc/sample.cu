@@ -6,23 +6,26 @@
 // or a sum of weights reach a target?  Sorting a row would answer them all;
 // the kernel instead narrows each question to the few tokens that decide it.
 //
-// One thread-block cluster holds one row in its shared memory, as integers
-// ordered like the logits, so the logits are read from HBM once.  The distance
-// from the largest logit, in base-2 units of the temperature, gives each token
-// one of 2048 bins; prefix sums over the bins' counts (and weights) bound where
-// each target lies.  When all that the filters can keep fits one CTA it is
-// gathered there, sorted, and every question is answered from running sums;
-// otherwise each question is answered alone: its bin is narrowed by further
-// histograms of its keys until what is left can be sorted, or is one value.
+// One thread-block cluster holds one row in its shared memory, so the logits
+// are read from HBM once.  The distance from the largest logit, in base-2
+// units of the temperature, gives each token one of 2048 bins; prefix sums
+// over the bins' counts (and weights) bound where each target lies.  When all
+// that the filters can keep fits one CTA it is gathered there, sorted, and
+// every question is answered from running sums; otherwise each question is
+// answered alone: its bin is narrowed by further histograms until what is left
+// can be sorted, or is one value.
 //
 // Weights are 2^(-distance) in 64-bit floating point, rounded to multiples of
 // 2^-shift of the largest, and added as 64-bit integers: sums do not depend on
 // the order, and are off by at most 2^-(shift + 1) per token (shift = 62 -
 // log2(vocab), 44 for 152k tokens), where f32 sums would move the borders.
+// The work per token, not HBM, is the bound: about 12 64-bit operations, a
+// few f32 ones and one or two shared-memory atomics.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 #include <stdint.h>
@@ -37,12 +40,13 @@ namespace cg = cooperative_groups;
 constexpr int kSmpThreads = 1024;
 constexpr int kSmpBins = 2048;
 constexpr int kSmpSort = 1024;       // tokens that one CTA sorts: one per thread
-constexpr int kSmpSlice = 42 * 1024; // tokens of one CTA: their keys fill its shared memory
+constexpr int kSmpSlice = 42 * 1024; // tokens of one CTA: their logits fill its shared memory
 constexpr int kSmpMaxCluster = 16;
 constexpr int kSmpMaxVocab = 1 << 19;
 constexpr float kBinsPerOctave = 32.0f;  // 2048 bins: 64 octaves
+constexpr int kExpTable = 64;
 constexpr float kTopPOff = 0.999999f, kGreedyBelow = 1e-6f;
-constexpr uint32_t kKeyNegInf = 0x007fffffu;
+constexpr uint32_t kKeyNegInf = 0x007fffffu, kKeyInf = 0xff800000u;
 
 struct SampleArgs {
   const void* logits;
@@ -56,67 +60,49 @@ struct SampleArgs {
   int32_t* kept;
 };
 
-// Integers in the order of the floats; NaN as -inf, -0 as 0.
+// Integers in the order of the floats (no NaN, no -0).
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (x != x) return kKeyNegInf;
-  const uint32_t u = __float_as_uint(x + 0.0f);
+  const uint32_t u = __float_as_uint(x);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// 2^t for t in [-64, 0]: the polynomial of e^(r ln 2) on |r| <= 1/2, its
-// Taylor series to the 12th power (the next term is below 2^-53 of it).
-__device__ __forceinline__ double exp2_poly(double t) {
-  const double big = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
-  const double kf = t + big;
-  const int k = __double2loint(kf);
-  const double r = (t - (kf - big)) * 0.69314718055994530942;
-  double p = 1.0 / 479001600.0;
-  p = fma(p, r, 1.0 / 39916800.0);
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return __hiloint2double(__double2hiint(p) + (k << 20), __double2loint(p));
-}
-
 struct Row {
-  uint32_t top;     // the largest key
-  double top_x, c;  // its value; log2(e) / T
-  float top_f, c_f;
+  float top, c_bins, d_max;  // the largest logit; bins per unit of distance; the distance of the last bin
+  double top64, c64;         // -kExpTable * log2(e) / T
   int shift;
+  const double* table;       // 2^(-j / kExpTable)
 
-  __device__ __forceinline__ double weight(uint32_t key) const {
-    if (key == top) return 1.0;
-    const double t = ((double)value_of(key) - top_x) * c;
-    return t >= -64.0 ? exp2_poly(t) : 0.0;
+  // weight * 2^shift, rounded.  With t = distance * 64 in base-2 units, t =
+  // 64 e + j + r, |r| <= 1/2: 2^(-t / 64) = 2^-e * table[j] * e^(-r ln 2 / 64),
+  // the last by its Taylor series to the 5th power (the next term is below
+  // 2^-54 of it).
+  __device__ __forceinline__ unsigned long long mass(float x) const {
+    const double t = ((double)x - top64) * c64;
+    if (!(t < (double)(kExpTable * 53))) return 0;  // below half a unit for every shift
+    const double big = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+    const double kf = t + big;
+    const int k = __double2loint(kf);
+    const double r = (t - (kf - big)) * (-0.69314718055994530942 / kExpTable);
+    double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    const double f = table[k & (kExpTable - 1)];
+    const double scaled = __hiloint2double(__double2hiint(f) + (shift - k / kExpTable) * (1 << 20), __double2loint(f));
+    return __double_as_longlong(fma(p, scaled, 4503599627370496.0)) & 0xfffffffffffffull;
   }
-  // weight * 2^shift, rounded (below 2^52)
-  __device__ __forceinline__ unsigned long long mass(uint32_t key) const {
-    const double w = weight(key);
-    return __double_as_longlong(w * (double)(1ll << shift) + 4503599627370496.0) & 0xfffffffffffffull;
+  __device__ __forceinline__ double weight(float x) const {
+    return exp2(((double)x - top64) * (c64 * (-1.0 / kExpTable)));
   }
-  // never decreases as the key falls: each step is a rounding of a monotone one
-  __device__ __forceinline__ int bin(uint32_t key) const {
-    const float d = (top_f - value_of(key)) * c_f * kBinsPerOctave;
-    return key == top ? 0 : d < (float)(kSmpBins - 1) ? (int)d : kSmpBins - 1;
+  // never decreases as x falls: each step is a rounding of a monotone one
+  __device__ __forceinline__ int bin(float x) const {
+    const float d = fminf(top - x, d_max);
+    return __float_as_int(fmaf(d, c_bins, 8388608.0f)) & 0xffff;  // 2^23: to the nearest whole number
   }
-};
-
-// A set of tokens: a bin (level 0), or the keys of [lo, hi].
-struct Part {
-  int by_bin;      // bins [bin0, bin1]; else keys
-  int bin0, bin1;
-  uint32_t lo, hi;
 };
 
 // A place in the order of the tokens.
@@ -133,6 +119,7 @@ struct alignas(16) Shared {
   uint32_t all_cnt[kSmpBins];          // the leader's: the cluster's histogram
   unsigned long long all_mass[kSmpBins];
   unsigned long long list[kSmpSort];   // gathered tokens, key in the upper half, ~index in the lower
+  double table[kExpTable];
   unsigned long long red[64];
   // exchanged between the CTAs of the cluster
   uint32_t top[kSmpMaxCluster], lo[kSmpMaxCluster], hi[kSmpMaxCluster];
@@ -142,7 +129,7 @@ struct alignas(16) Shared {
   int word;
   // the leader's decision, which every CTA reads
   int found_bin, found_cnt, above_cnt;
-  unsigned long long above_mass;
+  unsigned long long above_mass, total;
   Place place;
 };
 
@@ -189,43 +176,15 @@ __device__ __forceinline__ unsigned long long block_sum(unsigned long long v, un
 
 struct Sampler {
   Shared& s;
-  uint32_t* keys;  // this CTA's tokens
-  int n, base;     // how many, the first one's index
+  const float* xs;  // this CTA's logits, -inf beyond n up to a multiple of 4
+  int n, base;      // how many, the first one's index
   int rank, size;
   Row row;
   cg::cluster_group cl;
+  bool level0;      // the leader holds the bins' histogram with weights
 
-  __device__ __forceinline__ bool in(const Part& p, uint32_t key) const {
-    if (p.by_bin) {
-      const int b = row.bin(key);
-      return b >= p.bin0 && b <= p.bin1 && key > kKeyNegInf;
-    }
-    return key >= p.lo && key <= p.hi;
-  }
-
-  // The cluster's histogram of a part, in the leader's all_cnt / all_mass: by
-  // bin, or by (hi - key) >> shift.
-  __device__ void histogram(const Part& p, int shift, bool masses) {
-    for (int b = threadIdx.x; b < kSmpBins; b += kSmpThreads) s.cnt[b] = s.mass_lo[b] = s.mass_hi[b] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kSmpThreads) {
-      const uint32_t key = keys[i];
-      if (key <= kKeyNegInf) continue;
-      int b;
-      if (p.by_bin) {
-        b = row.bin(key);
-      } else {
-        if (key < p.lo || key > p.hi) continue;
-        b = (int)((p.hi - key) >> shift);
-      }
-      atomicAdd(&s.cnt[b], 1u);
-      if (masses) {
-        const unsigned long long q = row.mass(key);
-        const uint32_t lo = (uint32_t)q, old = atomicAdd(&s.mass_lo[b], lo);
-        const uint32_t up = (uint32_t)(q >> 32) + (old + lo < old ? 1u : 0u);
-        if (up) atomicAdd(&s.mass_hi[b], up);
-      }
-    }
+  // Adds the CTAs' histograms into the leader's all_cnt / all_mass.
+  __device__ void add_up(bool masses) {
     cl.sync();
     // each CTA adds its share of the bins over the cluster
     Shared* lead = cl.map_shared_rank(&s, 0);
@@ -242,6 +201,84 @@ struct Sampler {
       lead->all_mass[b] = m;
     }
     cl.sync();
+  }
+
+  __device__ __forceinline__ void clear(bool masses) {
+    for (int b = threadIdx.x; b < kSmpBins; b += kSmpThreads) {
+      s.cnt[b] = 0;
+      if (masses) s.mass_lo[b] = s.mass_hi[b] = 0;
+    }
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ void count(int b, unsigned long long q) {
+    atomicAdd(&s.cnt[b], 1u);
+    const uint32_t lo = (uint32_t)q, old = atomicAdd(&s.mass_lo[b], lo);
+    const uint32_t up = (uint32_t)(q >> 32) + (old + lo < old ? 1u : 0u);
+    if (up) atomicAdd(&s.mass_hi[b], up);
+  }
+
+  // The bins' counts, and the sum of this thread's weights if asked for.
+  template <bool kWeights>
+  __device__ __forceinline__ unsigned long long counts() {
+    clear(false);
+    unsigned long long z = 0;
+    for (int i = threadIdx.x * 4; i < n; i += kSmpThreads * 4) {
+      const float4 v = *reinterpret_cast<const float4*>(xs + i);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (x[j] > -INFINITY) atomicAdd(&s.cnt[row.bin(x[j])], 1u);
+        if (kWeights) z += row.mass(x[j]);
+      }
+    }
+    add_up(false);
+    level0 = false;
+    return z;
+  }
+
+  // The bins' counts and weights.
+  __device__ void histogram() {
+    clear(true);
+    for (int i = threadIdx.x * 4; i < n; i += kSmpThreads * 4) {
+      const float4 v = *reinterpret_cast<const float4*>(xs + i);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (x[j] > -INFINITY) count(row.bin(x[j]), row.mass(x[j]));
+    }
+    add_up(true);
+    level0 = true;
+  }
+
+  // The same of the keys in [lo, hi], by (hi - key) >> shift.
+  __device__ void histogram_of(uint32_t lo, uint32_t hi, int shift) {
+    clear(true);
+    for (int i = threadIdx.x; i < n; i += kSmpThreads) {
+      const uint32_t key = key_of(xs[i]);
+      if (key >= lo && key <= hi) count((int)((hi - key) >> shift), row.mass(xs[i]));
+    }
+    add_up(true);
+    level0 = false;
+  }
+
+  // The smallest key whose bin is at most b.  Block-wide; every CTA of the
+  // cluster finds the same.
+  __device__ uint32_t first_key(int b) {
+    const uint32_t top = key_of(row.top);
+    uint32_t at = 0;  // keys below `at` are in later bins
+#pragma unroll 1
+    for (int sh = 22; sh >= 0; sh = sh > 2 ? sh - 10 : sh - 3) {
+      const unsigned long long key = at + ((unsigned long long)threadIdx.x << sh);
+      const bool in = key > top || (key > kKeyNegInf && row.bin(value_of((uint32_t)key)) <= b);
+      const int out = kSmpThreads - __syncthreads_count(in);  // the candidates before the first that is in
+      if (out) at += (uint32_t)(out - 1) << sh;
+      if (sh == 2) {  // the last four keys, one after the other
+        while (at <= kKeyNegInf || (at <= top && row.bin(value_of(at)) > b)) ++at;
+        break;
+      }
+    }
+    return at;
   }
 
   // The leader's bin where the running count reaches `count`, or (count == 0)
@@ -287,20 +324,24 @@ struct Sampler {
     __syncthreads();
   }
 
-  // Gathers a part (at most kSmpSort tokens) into the leader's list, sorted.
-  __device__ void gather(const Part& p) {
+  // Gathers the tokens with logits in [lo, hi] (at most kSmpSort) into the
+  // leader's list, sorted.
+  __device__ void gather(float lo, float hi) {
     Shared* lead = cl.map_shared_rank(&s, 0);
     if (rank == 0) {
       s.list[threadIdx.x] = 0;
       if (threadIdx.x == 0) s.list_n = 0;
     }
     cl.sync();
-    for (int i = threadIdx.x; i < n; i += kSmpThreads) {
-      const uint32_t key = keys[i];
-      if (key > kKeyNegInf && in(p, key)) {
-        const int at = atomicAdd(&lead->list_n, 1);
-        if (at < kSmpSort) lead->list[at] = ((unsigned long long)key << 32) | (uint32_t)~(base + i);
-      }
+    for (int i = threadIdx.x * 4; i < n; i += kSmpThreads * 4) {
+      const float4 v = *reinterpret_cast<const float4*>(xs + i);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (x[j] >= lo && x[j] <= hi) {
+          const int at = atomicAdd(&lead->list_n, 1);
+          if (at < kSmpSort) lead->list[at] = ((unsigned long long)key_of(x[j]) << 32) | (uint32_t)~(base + i + j);
+        }
     }
     cl.sync();
     if (rank != 0) return;
@@ -335,7 +376,7 @@ struct Sampler {
   __device__ __forceinline__ void sums(uint32_t& key, unsigned long long& q, unsigned long long& mass) {
     const unsigned long long v = s.list[threadIdx.x];
     key = (uint32_t)(v >> 32);
-    q = v ? row.mass(key) : 0;
+    q = v ? row.mass(value_of(key)) : 0;
     unsigned long long c = 0, m = q;
     scan2(c, m, s.red);
     mass = s.above_mass + m;
@@ -346,59 +387,38 @@ struct Sampler {
   // CTA.  with_index: also the token's index.
   __device__ Place find(unsigned long long count, unsigned long long mass, bool with_index) {
     Shared* lead = cl.map_shared_rank(&s, 0);
-    Part p{1, 0, kSmpBins - 1, 0, 0};
-    int shift = 0;
-    if (rank == 0 && threadIdx.x == 0) s.above_cnt = 0, s.above_mass = 0;
-    for (int level = 0;; ++level) {
-      histogram(p, shift, true);
-      if (rank == 0) find_bin(count, mass);
-      cl.sync();
-      const int bin = lead->found_bin, cnt = lead->found_cnt;
-      Part q = p;
-      if (p.by_bin) {
-        q.bin0 = q.bin1 = bin;
-      } else {
-        q.hi = p.hi - ((uint32_t)bin << shift);
-        const uint32_t span = (1u << shift) - 1;
-        q.lo = q.hi - p.lo > span ? q.hi - span : p.lo;
-      }
-      if (cnt <= kSmpSort) {
-        gather(q);
-        if (rank == 0) {
-          uint32_t key;
-          unsigned long long w, sum;
-          sums(key, w, sum);
-          const int left = s.list_n;
-          const bool before = (int)threadIdx.x < left &&
-                              (count ? s.above_cnt + threadIdx.x + 1 < count : sum < mass);
-          const int at = min(__syncthreads_count(before), left - 1);
-          if ((int)threadIdx.x == at)
-            s.place = Place{s.above_cnt + at + 1, sum, key, (int)~(uint32_t)s.list[at]};
-        }
-        break;
-      }
-      // the keys that the bin really holds
-      uint32_t lo = 0xffffffffu, hi = 0;
-      for (int i = threadIdx.x; i < n; i += kSmpThreads) {
-        const uint32_t key = keys[i];
-        if (key > kKeyNegInf && in(q, key)) lo = min(lo, key), hi = max(hi, key);
-      }
-      lo = __reduce_min_sync(0xffffffffu, lo);
-      hi = __reduce_max_sync(0xffffffffu, hi);
+    if (!level0) histogram();
+    if (rank == 0) {
+      if (threadIdx.x == 0) s.above_cnt = 0, s.above_mass = 0;
       __syncthreads();
-      if ((threadIdx.x & 31) == 0) s.red[threadIdx.x >> 5] = ((unsigned long long)hi << 32) | lo;
+      find_bin(count, mass);
+    }
+    cl.sync();
+    int bin = lead->found_bin, cnt = lead->found_cnt;
+    uint32_t lo = first_key(bin), hi = bin ? first_key(bin - 1) - 1 : key_of(row.top);
+    while (cnt > kSmpSort) {
+      // the keys that are really there
+      uint32_t l = 0xffffffffu, h = 0;
+      for (int i = threadIdx.x; i < n; i += kSmpThreads) {
+        const uint32_t key = key_of(xs[i]);
+        if (key >= lo && key <= hi) l = min(l, key), h = max(h, key);
+      }
+      l = __reduce_min_sync(0xffffffffu, l);
+      h = __reduce_max_sync(0xffffffffu, h);
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) s.red[threadIdx.x >> 5] = ((unsigned long long)h << 32) | l;
       __syncthreads();
       if ((int)threadIdx.x < size) {
-        for (int w = 0; w < kSmpThreads / 32; ++w) lo = min(lo, (uint32_t)s.red[w]), hi = max(hi, (uint32_t)(s.red[w] >> 32));
+        for (int w = 0; w < kSmpThreads / 32; ++w) l = min(l, (uint32_t)s.red[w]), h = max(h, (uint32_t)(s.red[w] >> 32));
         Shared* o = cl.map_shared_rank(&s, threadIdx.x);
-        o->lo[rank] = lo;
-        o->hi[rank] = hi;
+        o->lo[rank] = l;
+        o->hi[rank] = h;
       }
       cl.sync();
       lo = 0xffffffffu, hi = 0;
       for (int r = 0; r < size; ++r) lo = min(lo, s.lo[r]), hi = max(hi, s.hi[r]);
       if (lo == hi) {  // equal logits: the place follows from their count, the index from their order
-        const unsigned long long w = row.mass(lo), above_m = lead->above_mass;
+        const unsigned long long w = row.mass(value_of(lo)), above_m = lead->above_mass;
         const int above_c = lead->above_cnt;
         unsigned long long m;
         if (count) m = count - above_c;
@@ -408,9 +428,24 @@ struct Sampler {
         cl.sync();  // the leader's words may change from here on
         return f;
       }
-      p = Part{0, 0, 0, lo, hi};
-      shift = max(0, 32 - __clz(hi - lo) - 11);
+      const int shift = max(0, 32 - __clz(hi - lo) - 11);
+      histogram_of(lo, hi, shift);
+      if (rank == 0) find_bin(count, mass);
       cl.sync();
+      bin = lead->found_bin, cnt = lead->found_cnt;
+      hi -= (uint32_t)bin << shift;
+      const uint32_t span = (1u << shift) - 1;
+      lo = hi - lo > span ? hi - span : lo;
+    }
+    gather(value_of(lo), value_of(hi));
+    if (rank == 0) {
+      uint32_t key;
+      unsigned long long w, sum;
+      sums(key, w, sum);
+      const int left = s.list_n;
+      const bool before = (int)threadIdx.x < left && (count ? s.above_cnt + threadIdx.x + 1 < count : sum < mass);
+      const int at = min(__syncthreads_count(before), left - 1);
+      if ((int)threadIdx.x == at) s.place = Place{s.above_cnt + at + 1, sum, key, (int)~(uint32_t)s.list[at]};
     }
     cl.sync();
     const Place f = lead->place;
@@ -422,7 +457,8 @@ struct Sampler {
   __device__ int nth(uint32_t key, int m) {
     const int per = (n + kSmpThreads - 1) / kSmpThreads, i0 = min(n, (int)threadIdx.x * per), i1 = min(n, i0 + per);
     unsigned long long mine = 0, none = 0;
-    for (int i = i0; i < i1; ++i) mine += keys[i] == key;
+    const float x = value_of(key);
+    for (int i = i0; i < i1; ++i) mine += xs[i] == x;
     unsigned long long incl = mine;
     scan2(incl, none, s.red);
     if (threadIdx.x == kSmpThreads - 1) s.word = (int)incl;
@@ -435,7 +471,7 @@ struct Sampler {
     if (m > lo && m <= lo + (int)mine) {
       int at = lo;
       for (int i = i0; i < i1; ++i)
-        if (keys[i] == key && ++at == m) {
+        if (xs[i] == x && ++at == m) {
           for (int r = 0; r < size; ++r) cl.map_shared_rank(&s, r)->word = base + i;
           break;
         }
@@ -460,20 +496,20 @@ template <typename T>
 __global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared& s = *reinterpret_cast<Shared*>(smem_raw);
-  uint32_t* keys = reinterpret_cast<uint32_t*>(smem_raw + sizeof(Shared));
+  float* xs = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
   cg::cluster_group cl = cg::this_cluster();
   const int size = (int)cl.num_blocks(), rank = (int)cl.block_rank(), b = blockIdx.x / size, tid = threadIdx.x;
   const int base = min(a.vocab, rank * a.slice), n = min(a.vocab, base + a.slice) - base;
   const T* x = static_cast<const T*>(a.logits) + b * a.stride + base;
 
-  // the row's keys, the largest of them and the number above -inf
-  uint32_t top = 0;
+  // the row (NaN as -inf, -0 as 0), the largest logit and the number above -inf
+  float high = -INFINITY;
   int valid = 0;
-  auto take = [&](int i, T v) {
-    const uint32_t k = key_of(as_float<T>(v));
-    keys[i] = k;
-    top = max(top, k);
-    valid += k > kKeyNegInf;
+  auto take = [&](float v) {
+    v = v == v ? v + 0.0f : -INFINITY;
+    high = fmaxf(high, v);
+    valid += v > -INFINITY;
+    return v;
   };
   constexpr int kVec = 16 / sizeof(T);
   int done = 0;
@@ -485,11 +521,17 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
       T v[kVec];
       memcpy(v, &u, 16);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) take(i + j, v[j]);
+      for (int j = 0; j < kVec; j += 4) {
+        const float4 f = make_float4(take(as_float<T>(v[j])), take(as_float<T>(v[j + 1])), take(as_float<T>(v[j + 2])),
+                                     take(as_float<T>(v[j + 3])));
+        *reinterpret_cast<float4*>(xs + i + j) = f;
+      }
     }
   }
-  for (int i = done + tid; i < n; i += kSmpThreads) take(i, x[i]);
-  top = __reduce_max_sync(0xffffffffu, top);
+  for (int i = done + tid; i < n; i += kSmpThreads) xs[i] = take(as_float<T>(x[i]));
+  if (tid < 4 && n + tid < (n + 3) / 4 * 4) xs[n + tid] = -INFINITY;
+  if (tid < kExpTable) s.table[tid] = exp2(-(double)tid / kExpTable);
+  uint32_t top = __reduce_max_sync(0xffffffffu, key_of(high));
   valid = __reduce_add_sync(0xffffffffu, valid);
   if ((tid & 31) == 0) s.red[tid >> 5] = ((unsigned long long)top << 32) | (unsigned)valid;
   cl.sync();  // red is written; every CTA of the cluster runs, so their shared memory can be
@@ -510,8 +552,10 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
   const bool use_p = p_in < kTopPOff, use_mp = mp_in > 0.0f;
   const double u = u_in > 0.0f ? (u_in < 1.0f ? (double)u_in : 1.0) : 0.0;
   const bool writer = rank == 0 && tid == 0;
-  Row row{top, 0.0, 0.0, 0.0f, 0.0f, a.shift};
-  Sampler smp{s, keys, n, base, rank, size, row, cl};
+  Row row{};
+  row.shift = a.shift;
+  row.table = s.table;
+  Sampler smp{s, xs, n, base, rank, size, row, cl, false};
 
   if (valid == 0) {  // nothing can be drawn; the same in every CTA
     if (writer) {
@@ -530,39 +574,46 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
     }
     return;
   }
-  row.top_f = value_of(top);
-  row.top_x = (double)row.top_f;
-  row.c = 1.4426950408889634074 / (double)temp;
-  row.c_f = (float)row.c;
+  if (top == kKeyInf) {  // the tokens at +inf share the weight, whatever the rest
+    for (int i = tid; i < n; i += kSmpThreads) {
+      const bool in = xs[i] == INFINITY;
+      xs[i] = in ? 0.0f : xs[i] > -INFINITY ? -FLT_MAX : -INFINITY;
+    }
+    top = key_of(0.0f);
+    __syncthreads();
+  }
+  row.top = value_of(top);
+  row.top64 = (double)row.top;
+  row.c64 = -1.4426950408889634074 / (double)temp * kExpTable;
+  row.c_bins = (float)(1.4426950408889634074 / (double)temp * kBinsPerOctave);
+  row.d_max = fminf((float)(kSmpBins - 1) / row.c_bins, FLT_MAX);
   smp.row = row;
 
-  // all weights' sum
-  unsigned long long z = 0;
   const int k = k_in > 0 && k_in < valid ? k_in : valid;
   const bool any = use_p || use_mp || k < valid;
-  if (use_p || !any) {
-    for (int i = tid; i < n; i += kSmpThreads) z += keys[i] > kKeyNegInf ? row.mass(keys[i]) : 0;
-    z = block_sum(z, s.red);
-    if (tid < size) cl.map_shared_rank(&s, tid)->z[rank] = z;
-    cl.sync();
-    z = 0;
-    for (int r = 0; r < size; ++r) z += s.z[r];
-  }
-  const unsigned long long p_mass = use_p ? (unsigned long long)ceil(fmax(0.0, (double)p_in) * (double)z) : 0;
-
+  Shared* lead = cl.map_shared_rank(&s, 0);
   int kept = valid;
-  unsigned long long norm = z;
+  unsigned long long norm;
   if (any) {
     // the bins that can hold kept tokens: up to where each filter's target is
     // surely reached, every token of a bin weighing at least the bin's end
-    Shared* lead = cl.map_shared_rank(&s, 0);
-    smp.histogram(Part{1, 0, kSmpBins - 1, 0, 0}, 0, false);
+    unsigned long long p_mass = 0;
+    if (use_p) {
+      unsigned long long z = block_sum(smp.counts<true>(), s.red);
+      if (tid < size) cl.map_shared_rank(&s, tid)->z[rank] = z;
+      cl.sync();
+      z = 0;
+      for (int r = 0; r < size; ++r) z += s.z[r];
+      p_mass = (unsigned long long)ceil(fmax(0.0, (double)p_in) * (double)z);
+    } else {
+      smp.counts<false>();
+    }
     if (rank == 0) {
       const int b0 = 2 * tid;
       const unsigned long long c0 = s.all_cnt[b0], c1 = s.all_cnt[b0 + 1];
-      // f32 rounding in bin() moves a token's distance by less than 2^-20 of it: half a bin at most
+      // bin b ends at b + 1/2, and f32 rounding moves a distance by less than 2^-20 of it
       const double unit = (double)(1ull << a.shift);
-      const double w0 = exp2((-(double)b0 - 1.5) / kBinsPerOctave), w1 = exp2((-(double)b0 - 2.5) / kBinsPerOctave);
+      const double w0 = exp2((-(double)b0 - 0.75) / kBinsPerOctave), w1 = exp2((-(double)b0 - 1.75) / kBinsPerOctave);
       unsigned long long c = c0 + c1;
       unsigned long long m = (unsigned long long)((double)c0 * w0 * unit) +
                              (b0 + 1 == kSmpBins - 1 ? 0ull : (unsigned long long)((double)c1 * w1 * unit));
@@ -579,14 +630,15 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
     cl.sync();
     const int last_bin = lead->found_bin, cnt = lead->found_cnt;
     if (cnt <= kSmpSort) {
+      const uint32_t lo = smp.first_key(last_bin);
       if (writer) s.above_cnt = 0, s.above_mass = 0;
-      smp.gather(Part{1, 0, last_bin, 0, 0});
+      smp.gather(value_of(lo), row.top);
       if (rank == 0) {
         uint32_t key;
         unsigned long long q, sum;
         smp.sums(key, q, sum);
         const bool here = tid < s.list_n;
-        const double w = here ? row.weight(key) : 0.0;
+        const double w = here ? row.weight(value_of(key)) : 0.0;
         int m = min(k, s.list_n);
         const int below = __syncthreads_count(here && sum < p_mass);
         if (use_p) m = min(m, below + 1);
@@ -612,7 +664,8 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
     if (use_p) kept = min(kept, smp.find(0, p_mass, false).n);
     if (use_mp) {
       int likely = 0;
-      for (int i = tid; i < n; i += kSmpThreads) likely += keys[i] > kKeyNegInf && row.weight(keys[i]) >= (double)mp_in;
+      for (int i = tid; i < n; i += kSmpThreads)
+        likely += xs[i] > -INFINITY && row.weight(xs[i]) >= (double)mp_in;
       const unsigned long long mine = block_sum((unsigned long long)likely, s.red);
       if (tid < size) cl.map_shared_rank(&s, tid)->z[rank] = mine;
       cl.sync();
@@ -623,13 +676,22 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
     }
     kept = max(kept, 1);
     norm = smp.find((unsigned long long)kept, 0, false).mass;
+  } else {
+    smp.histogram();
+    if (rank == 0) {
+      const unsigned long long z = block_sum(s.all_mass[tid] + s.all_mass[kSmpThreads + tid], s.red);
+      if (tid == 0) s.total = z;
+    }
+    cl.sync();
+    norm = lead->total;
   }
   const unsigned long long target = (unsigned long long)ceil(u * (double)norm);
   Place f = smp.find(0, target < norm ? target : norm, true);
   if (f.n > kept) f = smp.find((unsigned long long)kept, 0, true);  // tokens of no weight at the end
   if (writer) {
     a.tokens[b] = f.index;
-    if (a.probs) a.probs[b] = (float)(row.weight(f.key) * (double)(1ull << a.shift) / (double)norm);
+    const double w = row.weight(value_of(f.key));
+    if (a.probs) a.probs[b] = (float)(w * (double)(1ull << a.shift) / (double)norm);
     if (a.kept) a.kept[b] = kept;
   }
 }
