@@ -37,10 +37,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSmpThreads = 1024;
+constexpr int kSmpThreads = 512;     // two CTAs per SM: one row's barriers pass behind another's arithmetic
 constexpr int kSmpBins = 2048;
-constexpr int kSmpSort = 1024;       // tokens that one CTA sorts: one per thread
-constexpr int kSmpSlice = 42 * 1024; // tokens of one CTA: their logits fill its shared memory
+constexpr int kSmpSort = 1024;       // tokens that one CTA sorts: two per thread
+constexpr int kSmpSlice = 47 * 1024; // tokens of one CTA at most: their logits fill its shared memory
+constexpr int kSmpHalf = 19 * 1024 + 512;  // tokens that leave room for a second CTA
 constexpr int kSmpMaxCluster = 16;
 constexpr int kSmpMaxVocab = 1 << 19;
 constexpr float kBinsPerOctave = 32.0f;  // 2048 bins: 64 octaves
@@ -113,65 +114,52 @@ struct Place {
   int index;                 // -1: not asked for
 };
 
+// The bin where a target is reached.
+struct Found {
+  int bin, cnt;              // its tokens
+  int above_cnt;             // those above it, and their weights
+  unsigned long long above_mass;
+};
+
 struct alignas(16) Shared {
-  uint32_t cnt[kSmpBins];              // this CTA's histogram
-  uint32_t mass_lo[kSmpBins], mass_hi[kSmpBins];
-  uint32_t all_cnt[kSmpBins];          // the leader's: the cluster's histogram
-  unsigned long long all_mass[kSmpBins];
+  // this CTA's histogram; after add_up its share of the bins holds the cluster's
+  uint32_t cnt[kSmpBins], mass_lo[kSmpBins], mass_hi[kSmpBins];
   unsigned long long list[kSmpSort];   // gathered tokens, key in the upper half, ~index in the lower
   double table[kExpTable];
-  unsigned long long red[64];
-  // exchanged between the CTAs of the cluster
-  uint32_t top[kSmpMaxCluster], lo[kSmpMaxCluster], hi[kSmpMaxCluster];
-  int valid[kSmpMaxCluster], same[kSmpMaxCluster];
-  unsigned long long z[kSmpMaxCluster];
-  int list_n;
-  int word;
-  // the leader's decision, which every CTA reads
-  int found_bin, found_cnt, above_cnt;
-  unsigned long long above_mass, total;
+  unsigned long long red[2][kSmpThreads / 32];
+  uint32_t top;
+  int valid, word, list_n;
+  unsigned long long mark;
+  // written by the other CTAs of the cluster
+  uint32_t lo[kSmpMaxCluster], hi[kSmpMaxCluster];
+  int same[kSmpMaxCluster];
+  unsigned long long z[kSmpMaxCluster], tot_c[kSmpMaxCluster], tot_m[kSmpMaxCluster];
+  Found found;
   Place place;
 };
 
-__device__ __forceinline__ unsigned long long shfl_up64(unsigned long long v, int o) {
-  return __shfl_up_sync(0xffffffffu, v, o);
-}
-
-// Inclusive block scan of (count, mass); red is the scratch.
-__device__ __forceinline__ void scan2(unsigned long long& c, unsigned long long& m, unsigned long long* red) {
+// Inclusive block scan of (c, m); tc and tm get the block's sums.
+__device__ __forceinline__ void scan2(Shared& s, unsigned long long& c, unsigned long long& m, unsigned long long& tc,
+                                      unsigned long long& tm) {
+  constexpr int kWarps = kSmpThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long cu = shfl_up64(c, o), mu = shfl_up64(m, o);
+    const unsigned long long cu = __shfl_up_sync(0xffffffffu, c, o), mu = __shfl_up_sync(0xffffffffu, m, o);
     if (lane >= o) c += cu, m += mu;
   }
-  if (lane == 31) red[warp] = c, red[32 + warp] = m;
+  if (lane == 31) s.red[0][warp] = c, s.red[1][warp] = m;
   __syncthreads();
-  if (warp == 0) {
-    unsigned long long a = red[lane], b = red[32 + lane];
+  unsigned long long bc = 0, bm = 0;
+  tc = tm = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long au = shfl_up64(a, o), bu = shfl_up64(b, o);
-      if (lane >= o) a += au, b += bu;
-    }
-    red[lane] = a, red[32 + lane] = b;
+  for (int w = 0; w < kWarps; ++w) {
+    const unsigned long long x = s.red[0][w], y = s.red[1][w];
+    if (w < warp) bc += x, bm += y;
+    tc += x, tm += y;
   }
+  c += bc, m += bm;
   __syncthreads();
-  if (warp) c += red[warp - 1], m += red[32 + warp - 1];
-  __syncthreads();
-}
-
-__device__ __forceinline__ unsigned long long block_sum(unsigned long long v, unsigned long long* red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  unsigned long long s = red[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  __syncthreads();
-  return s;
 }
 
 struct Sampler {
@@ -181,28 +169,11 @@ struct Sampler {
   int rank, size;
   Row row;
   cg::cluster_group cl;
-  bool level0;      // the leader holds the bins' histogram with weights
+  bool level0;      // the shares hold the bins' histogram with weights
 
-  // Adds the CTAs' histograms into the leader's all_cnt / all_mass.
-  __device__ void add_up(bool masses) {
-    cl.sync();
-    // each CTA adds its share of the bins over the cluster
-    Shared* lead = cl.map_shared_rank(&s, 0);
-    const int share = kSmpBins / size;
-    for (int b = rank * share + (int)threadIdx.x; b < (rank + 1) * share; b += kSmpThreads) {
-      uint32_t c = 0;
-      unsigned long long m = 0;
-      for (int r = 0; r < size; ++r) {
-        const Shared* o = cl.map_shared_rank(&s, r);
-        c += o->cnt[b];
-        if (masses) m += ((unsigned long long)o->mass_hi[b] << 32) + o->mass_lo[b];
-      }
-      lead->all_cnt[b] = c;
-      lead->all_mass[b] = m;
-    }
-    cl.sync();
-  }
+  __device__ __forceinline__ Shared* of(int r) const { return cl.map_shared_rank(&s, r); }
 
+  // ---- histograms ----
   __device__ __forceinline__ void clear(bool masses) {
     for (int b = threadIdx.x; b < kSmpBins; b += kSmpThreads) {
       s.cnt[b] = 0;
@@ -210,12 +181,29 @@ struct Sampler {
     }
     __syncthreads();
   }
-
   __device__ __forceinline__ void count(int b, unsigned long long q) {
     atomicAdd(&s.cnt[b], 1u);
     const uint32_t lo = (uint32_t)q, old = atomicAdd(&s.mass_lo[b], lo);
     const uint32_t up = (uint32_t)(q >> 32) + (old + lo < old ? 1u : 0u);
     if (up) atomicAdd(&s.mass_hi[b], up);
+  }
+  // Each CTA adds its share of the bins over the cluster, in place: nobody
+  // else reads those here.
+  __device__ __forceinline__ void add_up(bool masses) {
+    cl.sync();
+    const int share = kSmpBins / size;
+    for (int b = rank * share + (int)threadIdx.x; b < (rank + 1) * share; b += kSmpThreads) {
+      uint32_t c = 0;
+      unsigned long long m = 0;
+      for (int r = 0; r < size; ++r) {
+        const Shared* o = of(r);
+        c += o->cnt[b];
+        if (masses) m += ((unsigned long long)o->mass_hi[b] << 32) + o->mass_lo[b];
+      }
+      s.cnt[b] = c;
+      if (masses) s.mass_lo[b] = (uint32_t)m, s.mass_hi[b] = (uint32_t)(m >> 32);
+    }
+    __syncthreads();
   }
 
   // The bins' counts, and the sum of this thread's weights if asked for.
@@ -232,13 +220,10 @@ struct Sampler {
         if (kWeights) z += row.mass(x[j]);
       }
     }
-    add_up(false);
-    level0 = false;
     return z;
   }
-
   // The bins' counts and weights.
-  __device__ void histogram() {
+  __device__ __forceinline__ void histogram() {
     clear(true);
     for (int i = threadIdx.x * 4; i < n; i += kSmpThreads * 4) {
       const float4 v = *reinterpret_cast<const float4*>(xs + i);
@@ -248,91 +233,105 @@ struct Sampler {
         if (x[j] > -INFINITY) count(row.bin(x[j]), row.mass(x[j]));
     }
     add_up(true);
+    totals();
     level0 = true;
   }
-
   // The same of the keys in [lo, hi], by (hi - key) >> shift.
-  __device__ void histogram_of(uint32_t lo, uint32_t hi, int shift) {
+  __device__ __forceinline__ void histogram_of(uint32_t lo, uint32_t hi, int shift) {
     clear(true);
     for (int i = threadIdx.x; i < n; i += kSmpThreads) {
       const uint32_t key = key_of(xs[i]);
       if (key >= lo && key <= hi) count((int)((hi - key) >> shift), row.mass(xs[i]));
     }
     add_up(true);
+    totals();
     level0 = false;
   }
 
-  // The smallest key whose bin is at most b.  Block-wide; every CTA of the
-  // cluster finds the same.
-  __device__ uint32_t first_key(int b) {
-    const uint32_t top = key_of(row.top);
-    uint32_t at = 0;  // keys below `at` are in later bins
-#pragma unroll 1
-    for (int sh = 22; sh >= 0; sh = sh > 2 ? sh - 10 : sh - 3) {
-      const unsigned long long key = at + ((unsigned long long)threadIdx.x << sh);
-      const bool in = key > top || (key > kKeyNegInf && row.bin(value_of((uint32_t)key)) <= b);
-      const int out = kSmpThreads - __syncthreads_count(in);  // the candidates before the first that is in
-      if (out) at += (uint32_t)(out - 1) << sh;
-      if (sh == 2) {  // the last four keys, one after the other
-        while (at <= kKeyNegInf || (at <= top && row.bin(value_of(at)) > b)) ++at;
-        break;
-      }
-    }
-    return at;
+  // ---- sums over the bins ----
+  // This thread's bins [b, e) of the CTA's share, and their count and weight.
+  __device__ __forceinline__ void my_bins(int& b, int& e) const {
+    const int share = kSmpBins / size, per = max(1, share / kSmpThreads);
+    b = rank * share + min(share, (int)threadIdx.x * per);
+    e = rank * share + min(share, ((int)threadIdx.x + 1) * per);
   }
-
-  // The leader's bin where the running count reaches `count`, or (count == 0)
-  // the running weight reaches `mass`; what is above it is added to
-  // s.above_cnt / s.above_mass.  The last non-empty bin if neither does.
-  // Leader's whole block.
-  __device__ void find_bin(unsigned long long count, unsigned long long mass) {
-    const int b0 = 2 * threadIdx.x;
-    const unsigned long long c0 = s.all_cnt[b0], c1 = s.all_cnt[b0 + 1], m0 = s.all_mass[b0], m1 = s.all_mass[b0 + 1];
-    unsigned long long c = c0 + c1, m = m0 + m1;
-    scan2(c, m, s.red);
-    const unsigned long long base_c = s.above_cnt, base_m = s.above_mass;
-    if (threadIdx.x == 0) s.found_bin = -1;
-    __syncthreads();
-    // first bin that reaches the target: exactly one thread and bin
-    const unsigned long long pc = base_c + c - c0 - c1, pm = base_m + m - m0 - m1;  // before this thread's bins
-    const bool r0 = count ? pc + c0 >= count : pm + m0 >= mass && c0;
-    const bool r1 = count ? pc + c0 + c1 >= count : pm + m0 + m1 >= mass && c1;
-    int mine = -1;
-    if (r0 && c0) mine = b0;
-    else if (r1 && c1) mine = b0 + 1;
-    // the least such bin over the block (a target of weight 0 is reached at once)
-    int least = mine < 0 ? INT_MAX : mine, last = c1 ? b0 + 1 : c0 ? b0 : -1;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-      last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
-    }
-    if ((threadIdx.x & 31) == 0) s.red[threadIdx.x >> 5] = (unsigned)least | ((unsigned long long)(unsigned)(last + 1) << 32);
-    __syncthreads();
-    least = INT_MAX, last = -1;
-    for (int w = 0; w < kSmpThreads / 32; ++w) {
-      least = min(least, (int)(uint32_t)s.red[w]);
-      last = max(last, (int)(s.red[w] >> 32) - 1);
-    }
-    const int bin = least == INT_MAX ? last : least;
-    if (bin >> 1 == (int)threadIdx.x) {
-      s.found_bin = bin;
-      s.found_cnt = (int)(bin & 1 ? c1 : c0);
-      s.above_cnt = (int)(pc + (bin & 1 ? c0 : 0));
-      s.above_mass = pm + (bin & 1 ? m0 : 0);
-    }
-    __syncthreads();
+  __device__ __forceinline__ unsigned long long bin_mass(int b) const {
+    return ((unsigned long long)s.mass_hi[b] << 32) + s.mass_lo[b];
   }
-
-  // Gathers the tokens with logits in [lo, hi] (at most kSmpSort) into the
-  // leader's list, sorted.
-  __device__ void gather(float lo, float hi) {
-    Shared* lead = cl.map_shared_rank(&s, 0);
-    if (rank == 0) {
-      s.list[threadIdx.x] = 0;
-      if (threadIdx.x == 0) s.list_n = 0;
+  // Tells every CTA this one's sums, and waits for theirs.
+  __device__ __forceinline__ void tell(unsigned long long c, unsigned long long m) {
+    if ((int)threadIdx.x < size) {
+      Shared* o = of(threadIdx.x);
+      o->tot_c[rank] = c;
+      o->tot_m[rank] = m;
     }
     cl.sync();
+  }
+  __device__ __forceinline__ void totals() {
+    int b, e;
+    my_bins(b, e);
+    unsigned long long c = 0, m = 0, tc, tm;
+    for (int i = b; i < e; ++i) c += s.cnt[i], m += bin_mass(i);
+    scan2(s, c, m, tc, tm);
+    tell(tc, tm);
+  }
+  __device__ __forceinline__ void before_me(unsigned long long& c, unsigned long long& m) const {
+    for (int r = 0; r < rank; ++r) c += s.tot_c[r], m += s.tot_m[r];
+  }
+  // The first bin where, on top of what is above, the running count reaches
+  // `count`, or (count == 0) the running weight reaches `mass` > 0.  The
+  // target lies above what is above and is reached, so one bin has it.
+  __device__ __forceinline__ Found find_bin(unsigned long long count, unsigned long long mass, int above_cnt,
+                                            unsigned long long above_mass) {
+    int b, e;
+    my_bins(b, e);
+    unsigned long long c = 0, m = 0, tc, tm, pc = above_cnt, pm = above_mass;
+    for (int i = b; i < e; ++i) c += s.cnt[i], m += bin_mass(i);
+    const unsigned long long c0 = c, m0 = m;
+    scan2(s, c, m, tc, tm);
+    before_me(pc, pm);
+    pc += c - c0, pm += m - m0;  // before this thread's bins
+    for (int i = b; i < e; ++i) {
+      const unsigned long long nc = pc + s.cnt[i], nm = pm + bin_mass(i);
+      if (count ? pc < count && nc >= count : pm < mass && nm >= mass)
+        for (int r = 0; r < size; ++r) of(r)->found = Found{i, (int)(nc - pc), (int)pc, pm};
+      pc = nc, pm = nm;
+    }
+    cl.sync();
+    return s.found;
+  }
+
+  // The smallest key whose bin is at most b.  Every thread of the cluster
+  // finds the same.
+  __device__ __forceinline__ uint32_t first_key(int b) const {
+    const uint32_t top = key_of(row.top);
+    auto in = [&](long long key) { return key > top || (key > kKeyNegInf && row.bin(value_of((uint32_t)key)) <= b); };
+    // where bin b should end, give or take f32 roundings; else a search of all keys
+    const int lane = threadIdx.x & 31;
+    const float guess = fmaxf(row.top - ((float)b + 0.5f) / row.c_bins, -FLT_MAX);
+    const long long g = (long long)key_of(guess + 0.0f) - 16;
+    const unsigned in32 = __ballot_sync(0xffffffffu, in(g + lane));
+    if (in32 != 0xffffffffu && in32 != 0u) return (uint32_t)(g + __ffs(in32) - 1);
+    uint32_t lo = kKeyNegInf, hi = top;  // lo is out, hi is in
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (in(mid)) hi = mid;
+      else lo = mid;
+    }
+    return hi;
+  }
+
+  // ---- gathering ----
+  __device__ __forceinline__ void empty_list() {  // the leader, before a cluster barrier
+    if (rank == 0) {
+      s.list[threadIdx.x] = s.list[threadIdx.x + kSmpThreads] = 0;
+      if (threadIdx.x == 0) s.list_n = 0;
+    }
+  }
+  // Gathers the tokens with logits in [lo, hi] (at most kSmpSort) into the
+  // leader's list, sorted: largest first, equal ones by index.
+  __device__ __forceinline__ void gather(float lo, float hi) {
+    Shared* lead = of(0);
     for (int i = threadIdx.x * 4; i < n; i += kSmpThreads * 4) {
       const float4 v = *reinterpret_cast<const float4*>(xs + i);
       const float x[4] = {v.x, v.y, v.z, v.w};
@@ -345,58 +344,70 @@ struct Sampler {
     }
     cl.sync();
     if (rank != 0) return;
-    // bitonic, largest first (all keys differ: the indexes do); empty places are 0
+    // bitonic, places tid and tid + 512 in a thread (all keys differ: the
+    // indexes do); empty places are 0
     int m = 32;
-    while (m < s.list_n) m <<= 1;
-    if (m > kSmpSort) m = kSmpSort;
-    const int i = threadIdx.x;
-    unsigned long long v = s.list[i];
+    while (m < s.list_n && m < kSmpSort) m <<= 1;
+    const int i0 = threadIdx.x, i1 = i0 + kSmpThreads;
+    unsigned long long v0 = s.list[i0], v1 = s.list[i1];
+    auto swap = [&](unsigned long long v, unsigned long long o, int i, int k, int j) {
+      const bool take_max = ((i & j) == 0) == ((i & k) == 0);  // runs with bit k clear descend
+      return take_max ? (o > v ? o : v) : (o < v ? o : v);
+    };
     for (int k = 2; k <= m; k <<= 1) {
       for (int j = k >> 1; j > 0; j >>= 1) {
-        unsigned long long o;
-        if (j >= 32) {
+        if (j == kSmpThreads) {
+          const unsigned long long a = v0, b = v1;
+          v0 = swap(a, b, i0, k, j);
+          v1 = swap(b, a, i1, k, j);
+        } else if (j >= 32) {
           __syncthreads();
-          s.list[i] = v;
+          s.list[i0] = v0;
+          s.list[i1] = v1;
           __syncthreads();
-          o = s.list[i ^ j];
+          v0 = swap(v0, s.list[i0 ^ j], i0, k, j);
+          v1 = swap(v1, s.list[i1 ^ j], i1, k, j);
         } else {
-          o = __shfl_xor_sync(0xffffffffu, v, j);
+          v0 = swap(v0, __shfl_xor_sync(0xffffffffu, v0, j), i0, k, j);
+          if (m > kSmpThreads) v1 = swap(v1, __shfl_xor_sync(0xffffffffu, v1, j), i1, k, j);
         }
-        const bool up = (i & k) != 0, low = (i & j) == 0;  // `up`: this run ascends
-        const bool take_max = low != up;
-        v = take_max ? (o > v ? o : v) : (o < v ? o : v);
       }
     }
     __syncthreads();
-    s.list[i] = v;
+    s.list[i0] = v0;
+    s.list[i1] = v1;
     __syncthreads();
   }
 
-  // The sorted list's token and running sums of this thread, on top of what is above.
-  __device__ __forceinline__ void sums(uint32_t& key, unsigned long long& q, unsigned long long& mass) {
-    const unsigned long long v = s.list[threadIdx.x];
-    key = (uint32_t)(v >> 32);
-    q = v ? row.mass(value_of(key)) : 0;
-    unsigned long long c = 0, m = q;
-    scan2(c, m, s.red);
-    mass = s.above_mass + m;
+  // The sorted list's tokens 2 tid and 2 tid + 1 and the running sums up to
+  // them, on top of what is above.  Leader's block.
+  __device__ __forceinline__ void sums(unsigned long long above, uint32_t (&key)[2], unsigned long long (&sum)[2]) {
+    unsigned long long q[2], c = 0, tc, tm;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const unsigned long long v = s.list[2 * threadIdx.x + j];
+      key[j] = (uint32_t)(v >> 32);
+      q[j] = v ? row.mass(value_of(key[j])) : 0;
+    }
+    unsigned long long m = q[0] + q[1];
+    scan2(s, c, m, tc, tm);
+    sum[1] = above + m;
+    sum[0] = sum[1] - q[1];
   }
+  // How many of the leader's list's tokens satisfy a condition.
+  __device__ __forceinline__ int how_many(bool a, bool b) const { return __syncthreads_count(a) + __syncthreads_count(b); }
 
   // The place where the running count reaches `count` (> 0), or the running
-  // weight reaches `mass`, over all tokens.  Cluster-wide; the answer in every
-  // CTA.  with_index: also the token's index.
-  __device__ Place find(unsigned long long count, unsigned long long mass, bool with_index) {
-    Shared* lead = cl.map_shared_rank(&s, 0);
+  // weight reaches `mass` (> 0, at most all), over all tokens.  Cluster-wide;
+  // with kFinal the leader alone has the answer, with the token's index; else
+  // every CTA has it, without.
+  template <bool kFinal>
+  __device__ __forceinline__ Place find(unsigned long long count, unsigned long long mass) {
     if (!level0) histogram();
-    if (rank == 0) {
-      if (threadIdx.x == 0) s.above_cnt = 0, s.above_mass = 0;
-      __syncthreads();
-      find_bin(count, mass);
-    }
-    cl.sync();
-    int bin = lead->found_bin, cnt = lead->found_cnt;
-    uint32_t lo = first_key(bin), hi = bin ? first_key(bin - 1) - 1 : key_of(row.top);
-    while (cnt > kSmpSort) {
+    empty_list();
+    Found f = find_bin(count, mass, 0, 0);
+    uint32_t lo = first_key(f.bin), hi = f.bin ? first_key(f.bin - 1) - 1 : key_of(row.top);
+    while (f.cnt > kSmpSort) {
       // the keys that are really there
       uint32_t l = 0xffffffffu, h = 0;
       for (int i = threadIdx.x; i < n; i += kSmpThreads) {
@@ -405,12 +416,12 @@ struct Sampler {
       }
       l = __reduce_min_sync(0xffffffffu, l);
       h = __reduce_max_sync(0xffffffffu, h);
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) s.red[threadIdx.x >> 5] = ((unsigned long long)h << 32) | l;
+      if ((threadIdx.x & 31) == 0) s.red[0][threadIdx.x >> 5] = ((unsigned long long)h << 32) | l;
       __syncthreads();
       if ((int)threadIdx.x < size) {
-        for (int w = 0; w < kSmpThreads / 32; ++w) l = min(l, (uint32_t)s.red[w]), h = max(h, (uint32_t)(s.red[w] >> 32));
-        Shared* o = cl.map_shared_rank(&s, threadIdx.x);
+        for (int w = 0; w < kSmpThreads / 32; ++w)
+          l = min(l, (uint32_t)s.red[0][w]), h = max(h, (uint32_t)(s.red[0][w] >> 32));
+        Shared* o = of(threadIdx.x);
         o->lo[rank] = l;
         o->hi[rank] = h;
       }
@@ -418,52 +429,53 @@ struct Sampler {
       lo = 0xffffffffu, hi = 0;
       for (int r = 0; r < size; ++r) lo = min(lo, s.lo[r]), hi = max(hi, s.hi[r]);
       if (lo == hi) {  // equal logits: the place follows from their count, the index from their order
-        const unsigned long long w = row.mass(value_of(lo)), above_m = lead->above_mass;
-        const int above_c = lead->above_cnt;
-        unsigned long long m;
-        if (count) m = count - above_c;
-        else m = w ? (mass > above_m ? (mass - above_m + w - 1) / w : 1) : 1;
-        m = m < 1 ? 1 : m > (unsigned long long)cnt ? (unsigned long long)cnt : m;
-        Place f{above_c + (int)m, above_m + m * w, lo, with_index ? nth(lo, (int)m) : -1};
-        cl.sync();  // the leader's words may change from here on
-        return f;
+        const unsigned long long w = row.mass(value_of(lo));
+        unsigned long long m = count ? count - f.above_cnt : w ? (mass - f.above_mass + w - 1) / w : 1;
+        m = m < 1 ? 1 : m > (unsigned long long)f.cnt ? (unsigned long long)f.cnt : m;
+        Place p{f.above_cnt + (int)m, f.above_mass + m * w, lo, kFinal ? nth(lo, (int)m) : -1};
+        cl.sync();  // lo and hi may be written again from here on
+        return p;
       }
       const int shift = max(0, 32 - __clz(hi - lo) - 11);
       histogram_of(lo, hi, shift);
-      if (rank == 0) find_bin(count, mass);
-      cl.sync();
-      bin = lead->found_bin, cnt = lead->found_cnt;
-      hi -= (uint32_t)bin << shift;
+      f = find_bin(count, mass, f.above_cnt, f.above_mass);
+      hi -= (uint32_t)f.bin << shift;
       const uint32_t span = (1u << shift) - 1;
       lo = hi - lo > span ? hi - span : lo;
     }
     gather(value_of(lo), value_of(hi));
     if (rank == 0) {
-      uint32_t key;
-      unsigned long long w, sum;
-      sums(key, w, sum);
-      const int left = s.list_n;
-      const bool before = (int)threadIdx.x < left && (count ? s.above_cnt + threadIdx.x + 1 < count : sum < mass);
-      const int at = min(__syncthreads_count(before), left - 1);
-      if ((int)threadIdx.x == at) s.place = Place{s.above_cnt + at + 1, sum, key, (int)~(uint32_t)s.list[at]};
+      uint32_t key[2];
+      unsigned long long sum[2];
+      sums(f.above_mass, key, sum);
+      const int left = s.list_n, i = 2 * threadIdx.x;
+      auto before = [&](int j) {
+        return i + j < left && (count ? (unsigned long long)(f.above_cnt + i + j + 1) < count : sum[j] < mass);
+      };
+      const int at = min(how_many(before(0), before(1)), left - 1);
+      if (at >> 1 == (int)threadIdx.x) {
+        const Place p{f.above_cnt + at + 1, sum[at & 1], key[at & 1], (int)~(uint32_t)s.list[at]};
+        if (kFinal) s.place = p;
+        else
+          for (int r = 0; r < size; ++r) of(r)->place = p;
+      }
+      if (kFinal) __syncthreads();
     }
-    cl.sync();
-    const Place f = lead->place;
-    cl.sync();
-    return f;
+    if (!kFinal) cl.sync();
+    const Place p = s.place;
+    if (!kFinal) cl.sync();
+    return p;
   }
 
-  // The index of the m-th token (from 1) whose key is `key`.
-  __device__ int nth(uint32_t key, int m) {
+  // The index of the m-th token (from 1) whose key is `key`; every CTA has it.
+  __device__ __forceinline__ int nth(uint32_t key, int m) {
     const int per = (n + kSmpThreads - 1) / kSmpThreads, i0 = min(n, (int)threadIdx.x * per), i1 = min(n, i0 + per);
-    unsigned long long mine = 0, none = 0;
+    unsigned long long mine = 0, none = 0, all, tm;
     const float x = value_of(key);
     for (int i = i0; i < i1; ++i) mine += xs[i] == x;
     unsigned long long incl = mine;
-    scan2(incl, none, s.red);
-    if (threadIdx.x == kSmpThreads - 1) s.word = (int)incl;
-    __syncthreads();
-    if ((int)threadIdx.x < size) cl.map_shared_rank(&s, threadIdx.x)->same[rank] = s.word;
+    scan2(s, incl, none, all, tm);
+    if ((int)threadIdx.x < size) of(threadIdx.x)->same[rank] = (int)all;
     cl.sync();
     int before = 0;
     for (int r = 0; r < rank; ++r) before += s.same[r];
@@ -472,7 +484,7 @@ struct Sampler {
       int at = lo;
       for (int i = i0; i < i1; ++i)
         if (xs[i] == x && ++at == m) {
-          for (int r = 0; r < size; ++r) cl.map_shared_rank(&s, r)->word = base + i;
+          for (int r = 0; r < size; ++r) of(r)->word = base + i;
           break;
         }
     }
@@ -493,7 +505,7 @@ template <>
 __device__ __forceinline__ float as_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 template <typename T>
-__global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
+__global__ void __launch_bounds__(kSmpThreads, 2) k_sample(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared& s = *reinterpret_cast<Shared*>(smem_raw);
   float* xs = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
@@ -533,18 +545,21 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
   if (tid < kExpTable) s.table[tid] = exp2(-(double)tid / kExpTable);
   uint32_t top = __reduce_max_sync(0xffffffffu, key_of(high));
   valid = __reduce_add_sync(0xffffffffu, valid);
-  if ((tid & 31) == 0) s.red[tid >> 5] = ((unsigned long long)top << 32) | (unsigned)valid;
-  cl.sync();  // red is written; every CTA of the cluster runs, so their shared memory can be
-  if (tid < size) {
+  if ((tid & 31) == 0) s.red[0][tid >> 5] = ((unsigned long long)top << 32) | (unsigned)valid;
+  __syncthreads();
+  if (tid == 0) {
     top = 0, valid = 0;
-    for (int w = 0; w < kSmpThreads / 32; ++w) top = max(top, (uint32_t)(s.red[w] >> 32)), valid += (int)(uint32_t)s.red[w];
-    Shared* o = cl.map_shared_rank(&s, tid);
-    o->top[rank] = top;
-    o->valid[rank] = valid;
+    for (int w = 0; w < kSmpThreads / 32; ++w)
+      top = max(top, (uint32_t)(s.red[0][w] >> 32)), valid += (int)(uint32_t)s.red[0][w];
+    s.top = top;
+    s.valid = valid;
   }
   cl.sync();
   top = 0, valid = 0;
-  for (int r = 0; r < size; ++r) top = max(top, s.top[r]), valid += s.valid[r];
+  for (int r = 0; r < size; ++r) {
+    const Shared* o = cl.map_shared_rank(&s, r);
+    top = max(top, o->top), valid += o->valid;
+  }
 
   const float temp = a.temperature ? a.temperature[b] : 1.0f;
   const int k_in = a.top_k ? a.top_k[b] : 0;
@@ -558,6 +573,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
   Sampler smp{s, xs, n, base, rank, size, row, cl, false};
 
   if (valid == 0) {  // nothing can be drawn; the same in every CTA
+    cl.sync();         // the others have read this one's words
     if (writer) {
       a.tokens[b] = 0;
       if (a.probs) a.probs[b] = 0.0f;
@@ -591,107 +607,101 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample(const SampleArgs a) {
 
   const int k = k_in > 0 && k_in < valid ? k_in : valid;
   const bool any = use_p || use_mp || k < valid;
-  Shared* lead = cl.map_shared_rank(&s, 0);
   int kept = valid;
-  unsigned long long norm;
+  unsigned long long norm = 0;
   if (any) {
     // the bins that can hold kept tokens: up to where each filter's target is
     // surely reached, every token of a bin weighing at least the bin's end
-    unsigned long long p_mass = 0;
+    unsigned long long p_mass = 1;
     if (use_p) {
-      unsigned long long z = block_sum(smp.counts<true>(), s.red);
-      if (tid < size) cl.map_shared_rank(&s, tid)->z[rank] = z;
-      cl.sync();
-      z = 0;
-      for (int r = 0; r < size; ++r) z += s.z[r];
-      p_mass = (unsigned long long)ceil(fmax(0.0, (double)p_in) * (double)z);
+      unsigned long long z = smp.counts<true>(), c = 0, tc, tm;
+      scan2(s, c, z, tc, tm);
+      if (tid < size) cl.map_shared_rank(&s, tid)->z[rank] = tm;
     } else {
       smp.counts<false>();
     }
-    if (rank == 0) {
-      const int b0 = 2 * tid;
-      const unsigned long long c0 = s.all_cnt[b0], c1 = s.all_cnt[b0 + 1];
-      // bin b ends at b + 1/2, and f32 rounding moves a distance by less than 2^-20 of it
-      const double unit = (double)(1ull << a.shift);
-      const double w0 = exp2((-(double)b0 - 0.75) / kBinsPerOctave), w1 = exp2((-(double)b0 - 1.75) / kBinsPerOctave);
-      unsigned long long c = c0 + c1;
-      unsigned long long m = (unsigned long long)((double)c0 * w0 * unit) +
-                             (b0 + 1 == kSmpBins - 1 ? 0ull : (unsigned long long)((double)c1 * w1 * unit));
-      scan2(c, m, s.red);
-      const int min_bin = use_mp ? (int)fmin((double)kSmpBins, fmax(0.0, -log2((double)mp_in)) * kBinsPerOctave + 2.0) : kSmpBins;
-      // pairs of bins before which some filter has ended
-      const bool open = !(c >= (unsigned long long)k) && !(use_p && m >= p_mass) && b0 + 2 <= min_bin;
-      const int pairs = __syncthreads_count(open);
-      if (tid == min(pairs, kSmpThreads - 1)) {
-        s.found_bin = b0 + 1;
-        s.found_cnt = (int)c;
-      }
+    smp.add_up(false);
+    if (use_p) {
+      unsigned long long z = 0;
+      for (int r = 0; r < size; ++r) z += s.z[r];
+      p_mass = (unsigned long long)fmax(1.0, ceil((double)p_in * (double)z));
     }
+    smp.empty_list();
+    int b0, b1;
+    smp.my_bins(b0, b1);
+    // bin b ends at b + 1/2, and f32 rounding moves a distance by less than 2^-20 of it
+    unsigned long long c = 0, m = 0, tc, tm, pc = 0, pm = 0;
+    for (int i = b0; i < b1; ++i) {
+      c += s.cnt[i];
+      if (use_p && i < kSmpBins - 1)
+        m += (unsigned long long)((double)s.cnt[i] * exp2((-(double)i - 0.75) / kBinsPerOctave) * (double)(1ull << a.shift));
+    }
+    const unsigned long long c0 = c, m0 = m;
+    scan2(s, c, m, tc, tm);
+    smp.tell(tc, tm);
+    smp.before_me(pc, pm);
+    pc += c - c0, pm += m - m0;  // before this thread's bins
+    const int min_bin =
+        use_mp ? (int)fmin((double)kSmpBins, fmax(0.0, -log2((double)mp_in)) * kBinsPerOctave + 2.0) : kSmpBins;
+    auto ended = [&](unsigned long long c, unsigned long long m, int b) {  // by the bins before b
+      return c >= (unsigned long long)k || (use_p && m >= p_mass) || b >= min_bin;
+    };
+    if (b0 < b1 && !ended(pc, pm, b0) && ended(pc + c0, pm + m0, b1))
+      for (int r = 0; r < size; ++r) cl.map_shared_rank(&s, r)->found = Found{b1 - 1, (int)(pc + c0), 0, 0};
     cl.sync();
-    const int last_bin = lead->found_bin, cnt = lead->found_cnt;
-    if (cnt <= kSmpSort) {
-      const uint32_t lo = smp.first_key(last_bin);
-      if (writer) s.above_cnt = 0, s.above_mass = 0;
-      smp.gather(value_of(lo), row.top);
+    const Found last = s.found;
+    if (last.cnt <= kSmpSort) {
+      smp.gather(value_of(smp.first_key(last.bin)), row.top);
       if (rank == 0) {
-        uint32_t key;
-        unsigned long long q, sum;
-        smp.sums(key, q, sum);
-        const bool here = tid < s.list_n;
-        const double w = here ? row.weight(value_of(key)) : 0.0;
-        int m = min(k, s.list_n);
-        const int below = __syncthreads_count(here && sum < p_mass);
-        if (use_p) m = min(m, below + 1);
-        const int likely = __syncthreads_count(here && w >= (double)mp_in);
-        if (use_mp) m = min(m, likely);
+        uint32_t key[2];
+        unsigned long long sum[2];
+        smp.sums(0, key, sum);
+        const int left = s.list_n;
+        const bool h0 = 2 * tid < left, h1 = 2 * tid + 1 < left;
+        int m = min(k, left);
+        if (use_p) m = min(m, smp.how_many(h0 && sum[0] < p_mass, h1 && sum[1] < p_mass) + 1);
+        if (use_mp)
+          m = min(m, smp.how_many(h0 && row.weight(value_of(key[0])) >= (double)mp_in,
+                                  h1 && row.weight(value_of(key[1])) >= (double)mp_in));
         m = max(m, 1);
+        if ((m - 1) >> 1 == tid) s.mark = sum[(m - 1) & 1];
         __syncthreads();
-        if (tid == m - 1) s.above_mass = sum;
-        __syncthreads();
-        const unsigned long long all = s.above_mass;
-        const unsigned long long target = (unsigned long long)ceil(u * (double)all);
-        const int at = min(__syncthreads_count(here && sum < target), m - 1);
-        if (tid == at) {
+        const unsigned long long all = s.mark, target = (unsigned long long)ceil(u * (double)all);
+        const int at = min(smp.how_many(h0 && sum[0] < target, h1 && sum[1] < target), m - 1);
+        if (at >> 1 == tid) {
           a.tokens[b] = (int)~(uint32_t)s.list[at];
-          if (a.probs) a.probs[b] = (float)(w * (double)(1ull << a.shift) / (double)all);
+          if (a.probs)
+            a.probs[b] = (float)(row.weight(value_of(key[at & 1])) * (double)(1ull << a.shift) / (double)all);
           if (a.kept) a.kept[b] = m;
         }
       }
       return;
     }
-    cl.sync();
+    cl.sync();  // found and tot may be written again from here on
     kept = k;
-    if (use_p) kept = min(kept, smp.find(0, p_mass, false).n);
+    if (use_p) kept = min(kept, smp.find<false>(0, p_mass).n);
     if (use_mp) {
-      int likely = 0;
-      for (int i = tid; i < n; i += kSmpThreads)
-        likely += xs[i] > -INFINITY && row.weight(xs[i]) >= (double)mp_in;
-      const unsigned long long mine = block_sum((unsigned long long)likely, s.red);
-      if (tid < size) cl.map_shared_rank(&s, tid)->z[rank] = mine;
+      unsigned long long likely = 0, c = 0, tc, tm;
+      for (int i = tid; i < n; i += kSmpThreads) likely += xs[i] > -INFINITY && row.weight(xs[i]) >= (double)mp_in;
+      scan2(s, c, likely, tc, tm);
+      if (tid < size) cl.map_shared_rank(&s, tid)->z[rank] = tm;
       cl.sync();
       unsigned long long all = 0;
       for (int r = 0; r < size; ++r) all += s.z[r];
       cl.sync();
-      kept = min(kept, (int)all);
+      kept = (int)min((unsigned long long)kept, all);
     }
     kept = max(kept, 1);
-    norm = smp.find((unsigned long long)kept, 0, false).mass;
+    norm = smp.find<false>((unsigned long long)kept, 0).mass;
   } else {
     smp.histogram();
-    if (rank == 0) {
-      const unsigned long long z = block_sum(s.all_mass[tid] + s.all_mass[kSmpThreads + tid], s.red);
-      if (tid == 0) s.total = z;
-    }
-    cl.sync();
-    norm = lead->total;
+    for (int r = 0; r < size; ++r) norm += s.tot_m[r];
   }
-  const unsigned long long target = (unsigned long long)ceil(u * (double)norm);
-  Place f = smp.find(0, target < norm ? target : norm, true);
-  if (f.n > kept) f = smp.find((unsigned long long)kept, 0, true);  // tokens of no weight at the end
+  const unsigned long long target = (unsigned long long)fmax(1.0, ceil(u * (double)norm));
+  const Place f = smp.find<true>(0, target < norm ? target : norm);
   if (writer) {
     a.tokens[b] = f.index;
-    const double w = row.weight(value_of(f.key));
-    if (a.probs) a.probs[b] = (float)(w * (double)(1ull << a.shift) / (double)norm);
+    if (a.probs) a.probs[b] = (float)(row.weight(value_of(f.key)) * (double)(1ull << a.shift) / (double)norm);
     if (a.kept) a.kept[b] = kept;
   }
 }
@@ -723,6 +733,7 @@ cudaError_t launch_sample(const SampleArgs& a, int cluster, cudaStream_t st) {
 
 static_assert(sizeof(Shared) % 16 == 0, "keys are 16-byte aligned");
 static_assert(sizeof(Shared) + (size_t)kSmpSlice * 4 <= 232448, "a slice fits shared memory");
+static_assert(2 * (sizeof(Shared) + (size_t)kSmpHalf * 4 + 1024) <= 228 * 1024, "two CTAs fit an SM");
 static_assert((long long)kSmpSlice * kSmpMaxCluster >= kSmpMaxVocab, "a cluster holds a row");
 
 }  // namespace
@@ -761,9 +772,10 @@ extern "C" int minicpmo_gpu_sample(const void* logits, int dtype, size_t rows, s
   a.tokens = tokens;
   a.probs = probs;
   a.kept = kept;
-  // CTAs per row: as few as hold it, more while there are SMs for them and
-  // each still has 4096 tokens
+  // CTAs per row: as few as hold it, two to an SM where 8 (the portable
+  // cluster) can; more while there are SMs for them and each has 4096 tokens
   int cluster = 1;
+  while (cluster < 8 && (size_t)cluster * kSmpHalf < vocab) cluster *= 2;
   while ((size_t)cluster * kSmpSlice < vocab) cluster *= 2;
   while (cluster < 8 && rows * cluster * 2 <= 148 && vocab >= (size_t)cluster * 2 * 4096) cluster *= 2;
   a.slice = (int)((vocab + cluster - 1) / cluster + 15) / 16 * 16;
