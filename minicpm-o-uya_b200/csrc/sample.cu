@@ -81,8 +81,8 @@ struct Row {
   // the last by its Taylor series to the 5th power (the next term is below
   // 2^-54 of it).
   __device__ __forceinline__ unsigned long long mass(float x) const {
-    const double t = ((double)x - top64) * c64;
-    if (!(t < (double)(kExpTable * 53))) return 0;  // below half a unit for every shift
+    // from 53 octaves on it is below half a unit for every shift
+    const double d = ((double)x - top64) * c64, t = d < (double)(kExpTable * 53) ? d : (double)(kExpTable * 53);
     const double big = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
     const double kf = t + big;
     const int k = __double2loint(kf);
@@ -169,7 +169,8 @@ struct Sampler {
   int rank, size;
   Row row;
   cg::cluster_group cl;
-  bool level0;      // the shares hold the bins' histogram with weights
+  bool level0;      // the shares hold the bins' histogram with counts and weights
+  unsigned long long ex_c, ex_m;  // of the last totals(): the share's count and weight before this thread's bins
 
   __device__ __forceinline__ Shared* of(int r) const { return cl.map_shared_rank(&s, r); }
 
@@ -181,8 +182,7 @@ struct Sampler {
     }
     __syncthreads();
   }
-  __device__ __forceinline__ void count(int b, unsigned long long q) {
-    atomicAdd(&s.cnt[b], 1u);
+  __device__ __forceinline__ void weigh(int b, unsigned long long q) {
     const uint32_t lo = (uint32_t)q, old = atomicAdd(&s.mass_lo[b], lo);
     const uint32_t up = (uint32_t)(q >> 32) + (old + lo < old ? 1u : 0u);
     if (up) atomicAdd(&s.mass_hi[b], up);
@@ -195,10 +195,19 @@ struct Sampler {
     for (int b = rank * share + (int)threadIdx.x; b < (rank + 1) * share; b += kSmpThreads) {
       uint32_t c = 0;
       unsigned long long m = 0;
-      for (int r = 0; r < size; ++r) {
-        const Shared* o = of(r);
-        c += o->cnt[b];
-        if (masses) m += ((unsigned long long)o->mass_hi[b] << 32) + o->mass_lo[b];
+      for (int r0 = 0; r0 < size; r0 += 8) {
+        uint32_t n[8], lo[8], hi[8];  // all loads before the sums
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          n[j] = lo[j] = hi[j] = 0;
+          if (r0 + j < size) {
+            const Shared* o = of(r0 + j);
+            n[j] = o->cnt[b];
+            if (masses) lo[j] = o->mass_lo[b], hi[j] = o->mass_hi[b];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c += n[j], m += ((unsigned long long)hi[j] << 32) + lo[j];
       }
       s.cnt[b] = c;
       if (masses) s.mass_lo[b] = (uint32_t)m, s.mass_hi[b] = (uint32_t)(m >> 32);
@@ -215,10 +224,11 @@ struct Sampler {
       const float4 v = *reinterpret_cast<const float4*>(xs + i);
       const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (x[j] > -INFINITY) atomicAdd(&s.cnt[row.bin(x[j])], 1u);
+      for (int j = 0; j < 4; ++j)
         if (kWeights) z += row.mass(x[j]);
-      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (x[j] > -INFINITY) atomicAdd(&s.cnt[row.bin(x[j])], 1u);
     }
     return z;
   }
@@ -228,9 +238,16 @@ struct Sampler {
     for (int i = threadIdx.x * 4; i < n; i += kSmpThreads * 4) {
       const float4 v = *reinterpret_cast<const float4*>(xs + i);
       const float x[4] = {v.x, v.y, v.z, v.w};
+      unsigned long long q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j] = row.mass(x[j]);  // apart from the atomics, to overlap
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (x[j] > -INFINITY) count(row.bin(x[j]), row.mass(x[j]));
+        if (x[j] > -INFINITY) {
+          const int b = row.bin(x[j]);
+          atomicAdd(&s.cnt[b], 1u);
+          weigh(b, q[j]);
+        }
     }
     add_up(true);
     totals();
@@ -241,7 +258,11 @@ struct Sampler {
     clear(true);
     for (int i = threadIdx.x; i < n; i += kSmpThreads) {
       const uint32_t key = key_of(xs[i]);
-      if (key >= lo && key <= hi) count((int)((hi - key) >> shift), row.mass(xs[i]));
+      if (key >= lo && key <= hi) {
+        const int b = (int)((hi - key) >> shift);
+        atomicAdd(&s.cnt[b], 1u);
+        weigh(b, row.mass(xs[i]));
+      }
     }
     add_up(true);
     totals();
@@ -272,7 +293,9 @@ struct Sampler {
     my_bins(b, e);
     unsigned long long c = 0, m = 0, tc, tm;
     for (int i = b; i < e; ++i) c += s.cnt[i], m += bin_mass(i);
+    ex_c = c, ex_m = m;
     scan2(s, c, m, tc, tm);
+    ex_c = c - ex_c, ex_m = m - ex_m;
     tell(tc, tm);
   }
   __device__ __forceinline__ void before_me(unsigned long long& c, unsigned long long& m) const {
@@ -285,12 +308,8 @@ struct Sampler {
                                             unsigned long long above_mass) {
     int b, e;
     my_bins(b, e);
-    unsigned long long c = 0, m = 0, tc, tm, pc = above_cnt, pm = above_mass;
-    for (int i = b; i < e; ++i) c += s.cnt[i], m += bin_mass(i);
-    const unsigned long long c0 = c, m0 = m;
-    scan2(s, c, m, tc, tm);
+    unsigned long long pc = above_cnt + ex_c, pm = above_mass + ex_m;
     before_me(pc, pm);
-    pc += c - c0, pm += m - m0;  // before this thread's bins
     for (int i = b; i < e; ++i) {
       const unsigned long long nc = pc + s.cnt[i], nm = pm + bin_mass(i);
       if (count ? pc < count && nc >= count : pm < mass && nm >= mass)
@@ -403,7 +422,6 @@ struct Sampler {
   // every CTA has it, without.
   template <bool kFinal>
   __device__ __forceinline__ Place find(unsigned long long count, unsigned long long mass) {
-    if (!level0) histogram();
     empty_list();
     Found f = find_bin(count, mass, 0, 0);
     uint32_t lo = first_key(f.bin), hi = f.bin ? first_key(f.bin - 1) - 1 : key_of(row.top);
@@ -570,7 +588,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) k_sample(const SampleArgs a) {
   Row row{};
   row.shift = a.shift;
   row.table = s.table;
-  Sampler smp{s, xs, n, base, rank, size, row, cl, false};
+  Sampler smp{s, xs, n, base, rank, size, row, cl, false, 0, 0};
 
   if (valid == 0) {  // nothing can be drawn; the same in every CTA
     cl.sync();         // the others have read this one's words
@@ -678,8 +696,12 @@ __global__ void __launch_bounds__(kSmpThreads, 2) k_sample(const SampleArgs a) {
       return;
     }
     cl.sync();  // found and tot may be written again from here on
+    smp.histogram();
     kept = k;
-    if (use_p) kept = min(kept, smp.find<false>(0, p_mass).n);
+    if (use_p) {
+      const Place p = smp.find<false>(0, p_mass);
+      if (p.n <= kept) kept = p.n, norm = p.mass;
+    }
     if (use_mp) {
       unsigned long long likely = 0, c = 0, tc, tm;
       for (int i = tid; i < n; i += kSmpThreads) likely += xs[i] > -INFINITY && row.weight(xs[i]) >= (double)mp_in;
@@ -689,10 +711,12 @@ __global__ void __launch_bounds__(kSmpThreads, 2) k_sample(const SampleArgs a) {
       unsigned long long all = 0;
       for (int r = 0; r < size; ++r) all += s.z[r];
       cl.sync();
-      kept = (int)min((unsigned long long)kept, all);
+      if (all < (unsigned long long)kept) kept = (int)all, norm = 0;
     }
     kept = max(kept, 1);
-    norm = smp.find<false>((unsigned long long)kept, 0).mass;
+    if (!smp.level0) smp.histogram();
+    if (!norm) norm = smp.find<false>((unsigned long long)kept, 0).mass;
+    if (!smp.level0) smp.histogram();
   } else {
     smp.histogram();
     for (int r = 0; r < size; ++r) norm += s.tot_m[r];
