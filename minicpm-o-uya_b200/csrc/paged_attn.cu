@@ -52,6 +52,11 @@ __device__ __forceinline__ bool paged_last(const PagedAttnArgs& a, const PagedPi
 // ---------------------------------------------------------------------
 // f32: FMAs
 // ---------------------------------------------------------------------
+// f32 products keep f32's accuracy only on the FMA units.  A block is 16 rows;
+// a thread has two rows x two keys of the scores and two rows x head_dim / 16
+// columns of the output, so shared memory gives each operand to 16 threads.
+// Shared-memory reads bound it (6 wavefronts per 16 FMAs of a warp), about
+// half of the FMA rate.  A warp copies 8 keys of a tile: one table entry each.
 constexpr int kSimtRows = 16, kSimtKeys = 32, kSimtThreads = 128;
 
 template <int HD>
@@ -63,13 +68,17 @@ struct SimtSmem {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kSimtThreads) k_paged_attn_f32(const PagedAttnArgs a) {
+constexpr int kSimtCtas = HD == 64 ? 4 : HD == 128 ? 3 : 1;  // per SM, by shared memory and registers
+
+template <int HD>
+__global__ void __launch_bounds__(kSimtThreads, kSimtCtas<HD>) k_paged_attn_f32(const PagedAttnArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   SimtSmem<HD>& s = *reinterpret_cast<SimtSmem<HD>*>(smem_raw);
   __shared__ PagedShared sched;
   __shared__ unsigned last_s;
   constexpr int kCols = HD / 16;  // accumulator columns of a thread, for each of its two rows
   const int tid = threadIdx.x, x = tid & 15, y = tid >> 4;  // rows 2y, 2y + 1
+  const int warp = tid >> 5, lane = tid & 31;
   const int block_tokens = kSimtRows / a.group;
   const float* qg = static_cast<const float*>(a.q);
   const float* kg = static_cast<const float*>(a.kc);
@@ -80,22 +89,26 @@ __global__ void __launch_bounds__(kSimtThreads) k_paged_attn_f32(const PagedAttn
   while (walk.next(a, &p)) {
     const int t0 = p.b * block_tokens, rows = min(block_tokens, p.req.n_new - t0) * a.group;
     const int seen = paged_seen(p.req, p.b, block_tokens);
-    auto load = [&](int tile, int st) {
-      for (int e = tid; e < kSimtKeys * HD / 4; e += kSimtThreads) {
-        const int key = e / (HD / 4), c = e % (HD / 4) * 4, pos = tile * kSimtKeys + key;
-        bool in = pos < seen;
-        long long at = 0;
-        if (in) {
-          const int id = a.table[p.r * a.table_stride + (pos >> a.page_shift)];
-          in = id >= 0 && id < a.n_pages;
-          if (in) at = id * a.page_stride + (pos & ((1 << a.page_shift) - 1)) * a.token_stride + p.h * a.head_stride + c;
-        }
+    const int32_t* table = a.table + p.r * a.table_stride;
+    auto page = [&](int tile) {  // of this warp's 8 keys of a tile
+      const int pos = tile * kSimtKeys + warp * 8;
+      return tile < p.tile1 && pos < seen ? table[pos >> a.page_shift] : -1;
+    };
+    auto load = [&](int tile, int st, int id) {
+      const bool there = id >= 0 && id < a.n_pages;
+      const long long base = there ? id * a.page_stride + p.h * a.head_stride : 0;
+#pragma unroll
+      for (int j = 0; j < HD / 16; ++j) {
+        const int e = lane + 32 * j, key = warp * 8 + e / (HD / 4), c = e % (HD / 4) * 4, pos = tile * kSimtKeys + key;
+        const bool in = there && pos < seen;
+        const long long at = in ? base + (pos & ((1 << a.page_shift) - 1)) * a.token_stride + c : 0;
         cp_async16(&s.k[st][key][c], kg + at, in);
         cp_async16(&s.v[st][key][c], vg + at, in);
       }
       cp_async_commit();
     };
-    load(p.tile0, 0);
+    load(p.tile0, 0, page(p.tile0));
+    int next_page = page(p.tile0 + 1);
     for (int e = tid; e < kSimtRows * HD / 4; e += kSimtThreads) {
       const int row = e / (HD / 4), c = e % (HD / 4) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -105,18 +118,19 @@ __global__ void __launch_bounds__(kSimtThreads) k_paged_attn_f32(const PagedAttn
       *reinterpret_cast<float4*>(&s.q[row][c]) = v;
     }
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[2][kCols];
-    int see[2];  // keys that each row sees
+    int see[2];  // keys that each row sees (rows without a token: all, so that they mask nothing)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = 2 * y + i;
-      see[i] = row < rows ? max(0, p.req.len - p.req.n_new + t0 + row / a.group + 1) : 0;
+      see[i] = row < rows ? max(0, p.req.len - p.req.n_new + t0 + row / a.group + 1) : INT_MAX;
 #pragma unroll
       for (int c = 0; c < kCols; ++c) acc[i][c] = 0.f;
     }
     for (int tile = p.tile0; tile < p.tile1; ++tile) {
       const int st = (tile - p.tile0) & 1, key0 = tile * kSimtKeys;
       if (tile + 1 < p.tile1) {
-        load(tile + 1, st ^ 1);
+        load(tile + 1, st ^ 1, next_page);
+        next_page = page(tile + 2);
         cp_async_wait<1>();
       } else {
         cp_async_wait<0>();
@@ -161,12 +175,7 @@ __global__ void __launch_bounds__(kSimtThreads) k_paged_attn_f32(const PagedAttn
         for (int c = 0; c < kCols; ++c) acc[i][c] *= corr;
       }
       __syncwarp();
-      const bool all = key0 + kSimtKeys <= see[0] && key0 + kSimtKeys <= see[1];
-#pragma unroll 4
-      for (int key = 0; key < kSimtKeys; ++key) {
-        float w0 = s.p[2 * y][key], w1 = s.p[2 * y + 1][key];
-        // a key that a row does not see adds nothing, whatever V holds there
-        const bool on0 = all || key0 + key < see[0], on1 = all || key0 + key < see[1];
+      auto add = [&](int key, float w0, float w1, bool on0, bool on1) {
 #pragma unroll
         for (int c = 0; c < kCols; c += 4) {
           const float4 v4 = *reinterpret_cast<const float4*>(&s.v[st][key][x * 4 + c * 16]);
@@ -183,6 +192,23 @@ __global__ void __launch_bounds__(kSimtThreads) k_paged_attn_f32(const PagedAttn
             acc[1][c + 3] = fmaf(w1, v4.w, acc[1][c + 3]);
           }
         }
+      };
+      const bool all = key0 + kSimtKeys <= see[0] && key0 + kSimtKeys <= see[1];
+      if (__all_sync(0xffffffffu, all)) {
+#pragma unroll 2
+        for (int key = 0; key < kSimtKeys; key += 4) {
+          const float4 w0 = *reinterpret_cast<const float4*>(&s.p[2 * y][key]);
+          const float4 w1 = *reinterpret_cast<const float4*>(&s.p[2 * y + 1][key]);
+          add(key, w0.x, w1.x, true, true);
+          add(key + 1, w0.y, w1.y, true, true);
+          add(key + 2, w0.z, w1.z, true, true);
+          add(key + 3, w0.w, w1.w, true, true);
+        }
+      } else {
+        // a key that a row does not see adds nothing, whatever V holds there
+#pragma unroll 1
+        for (int key = 0; key < kSimtKeys; ++key)
+          add(key, s.p[2 * y][key], s.p[2 * y + 1][key], key0 + key < see[0], key0 + key < see[1]);
       }
       __syncthreads();
     }
@@ -581,7 +607,7 @@ cudaError_t launch_f32(const PagedAttnArgs& a, cudaStream_t st) {
   int sms = 0;
   const cudaError_t e = ready<k_paged_attn_f32<HD>>(sizeof(SimtSmem<HD>), &sms);
   if (e != cudaSuccess) return e;
-  const int ctas = HD == 256 ? sms : 2 * sms;  // residents by shared memory
+  const int ctas = kSimtCtas<HD> * sms;
   k_paged_attn_f32<HD><<<ctas < kPagedMaxCtas ? ctas : kPagedMaxCtas, kSimtThreads, sizeof(SimtSmem<HD>), st>>>(a);
   return cudaGetLastError();
 }
