@@ -294,6 +294,15 @@ MINICPMO_API int minicpmo_gpu_context_qwen3_forward_batch(void *handle, size_t n
 MINICPMO_API int minicpmo_gpu_context_qwen3_decode_batch(void *handle, size_t n_seq, const uint32_t *first_tokens,
                                             const uint32_t *first_positions, size_t n_steps, uint32_t *tokens_out,
                                             char *error, size_t error_cap);
+/* One token per sequence drawn from the logits of the last batched step that
+ * computed them (forward_batch, decode_batch), as minicpmo_gpu_sample does;
+ * host arrays [n_seq], each parameter NULL for off, out_probs and out_kept may
+ * be NULL.  Unlike minicpmo_gpu_context_qwen3_sample it draws for every
+ * vocabulary, from given random numbers. */
+MINICPMO_API int minicpmo_gpu_context_qwen3_sample_batch(void *handle, size_t n_seq, const float *temperature,
+                                            const int32_t *top_k, const float *top_p, const float *min_p,
+                                            const float *uniform, uint32_t *out_tokens, float *out_probs,
+                                            int32_t *out_kept, char *error, size_t error_cap);
 /* Device time of n_steps batched decode steps (graph replays, CUDA events
  * on the context stream); total_ms over all steps. */
 MINICPMO_API int minicpmo_gpu_context_qwen3_time_decode_batch(void *handle, size_t n_seq, const uint32_t *first_tokens,

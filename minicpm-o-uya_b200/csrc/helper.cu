@@ -73,6 +73,8 @@ struct BatchState {
   unsigned* attn_counters = nullptr;
   StepState* st = nullptr;       // [B]
   StepState* st_host = nullptr;  // pinned [B]
+  uint32_t* smp = nullptr;  // sample_batch: 5 parameters and 3 results, [B] each
+  bool has_logits = false;  // a step that computed them has run
   float* am_scratch = nullptr;
   unsigned* am_counter = nullptr;
   int* history = nullptr;  // [B][history_cap]
@@ -507,7 +509,7 @@ void free_batch(BatchState* b) {
   for (auto& e : b->exec)
     if (e) cudaGraphExecDestroy(e), e = nullptr;
   void* bufs[] = {b->hidden, b->qkv, b->attn, b->gu, b->logits, b->x16, b->part, b->cnt, b->kc, b->vc,
-                  b->attn_partial, b->attn_counters, b->st, b->am_scratch, b->am_counter, b->history, b->gbuf};
+                  b->attn_partial, b->attn_counters, b->st, b->am_scratch, b->am_counter, b->history, b->smp, b->gbuf};
   for (void* p : bufs)
     if (p) cudaFree(p);
   if (b->st_host) cudaFreeHost(b->st_host);
@@ -1064,6 +1066,7 @@ int bind_batch(Ctx* c, Model& m, char* err, size_t cap) {
       {(void**)&b.am_scratch, (size_t)B * b.am_grid * 3 * 4},
       {(void**)&b.am_counter, (size_t)B * 4},
       {(void**)&b.history, (size_t)B * b.history_cap * 4},
+      {(void**)&b.smp, (size_t)B * 8 * 4},
   };
   for (auto& a : allocs) {
     if (!cuda_ok(c, cudaMalloc(a.p, a.bytes), "qwen3_bind_batch_malloc", err, cap)) return 0;
@@ -1123,6 +1126,7 @@ int run_batch(Ctx* c, Model& m, const uint32_t* tokens, const uint32_t* pos, int
     ok = cuda_ok(c, cudaMemcpyAsync(b.st_host, b.st, b.B * sizeof(StepState), cudaMemcpyDeviceToHost, c->stream),
                  "batch_state_d2h", err, cap);
   if (ok) ok = cuda_ok(c, cudaStreamSynchronize(c->stream), "batch_sync", err, cap);
+  if (ok && which == 0 && steps > 0) b.has_logits = true;
   for (int i = 0; ok && i < b.B; ++i)
     if (b.st_host[i].err) ok = fail(c, err, cap, "error: qwen3 batch: a device-side check failed (a bounded wait gave up, or a position outside the cache)");
   if (ok && total_ms) cudaEventElapsedTime(total_ms, e0, e1);
@@ -3079,6 +3083,43 @@ int minicpmo_gpu_context_qwen3_decode_batch(void* handle, size_t n_seq, const ui
         return 0;
     c->stats.device_to_host_bytes += (size_t)b.B * n_steps * 4;
   }
+  return 1;
+}
+
+int minicpmo_gpu_context_qwen3_sample_batch(void* handle, size_t n_seq, const float* temperature, const int32_t* top_k,
+                                            const float* top_p, const float* min_p, const float* uniform,
+                                            uint32_t* out_tokens, float* out_probs, int32_t* out_kept, char* error,
+                                            size_t error_cap) {
+  Ctx* c = (Ctx*)handle;
+  if (!c) return copy_error(error, error_cap, "error: null gpu context"), 0;
+  DeviceGuard g(c);
+  if (!c->model || !c->model->batch) return fail(c, error, error_cap, "error: qwen3 sample_batch: no batched model bound");
+  Model& m = *c->model;
+  BatchState& b = *m.batch;
+  if (n_seq != (size_t)b.B || !uniform || !out_tokens)
+    return fail(c, error, error_cap, "error: qwen3 sample_batch: n_seq=%zu must equal max_batch=%d", n_seq, b.B);
+  if (!b.has_logits) return fail(c, error, error_cap, "error: qwen3 sample_batch: no step has computed logits");
+  const size_t bytes = n_seq * 4;
+  const void* in[5] = {temperature, top_k, top_p, min_p, uniform};
+  const uint32_t* dev[5];
+  for (int i = 0; i < 5; ++i) {
+    dev[i] = in[i] ? b.smp + i * n_seq : nullptr;
+    if (in[i] && !cuda_ok(c, cudaMemcpyAsync(b.smp + i * n_seq, in[i], bytes, cudaMemcpyHostToDevice, c->stream),
+                          "sample_batch_h2d", error, error_cap))
+      return 0;
+  }
+  uint32_t* out = b.smp + 5 * n_seq;
+  char msg[256] = "";
+  if (!minicpmo_gpu_sample(b.logits, kF32, n_seq, m.cfg.vocab, m.cfg.vocab, (const float*)dev[0], (const int32_t*)dev[1],
+                           (const float*)dev[2], (const float*)dev[3], (const float*)dev[4], (int32_t*)out,
+                           (float*)(out + n_seq), (int32_t*)(out + 2 * n_seq), c->stream, msg, sizeof(msg)))
+    return fail(c, error, error_cap, "%s", msg);
+  void* host[3] = {out_tokens, out_probs, out_kept};
+  for (int i = 0; i < 3; ++i)
+    if (host[i] && !cuda_ok(c, cudaMemcpyAsync(host[i], out + i * n_seq, bytes, cudaMemcpyDeviceToHost, c->stream),
+                            "sample_batch_d2h", error, error_cap))
+      return 0;
+  if (!cuda_ok(c, cudaStreamSynchronize(c->stream), "sample_batch_sync", error, error_cap)) return 0;
   return 1;
 }
 

@@ -161,6 +161,7 @@ SIGNATURES = {
     "minicpmo_gpu_context_time_matmul_q8_0_batch": (i32, [vp, vp, sz, i32, fptr] + E),
     "minicpmo_gpu_context_qwen3_forward_batch": (i32, [vp, sz, u32ptr, u32ptr, i32, u32ptr, fptr, fptr] + E),
     "minicpmo_gpu_context_qwen3_decode_batch": (i32, [vp, sz, u32ptr, u32ptr, sz, u32ptr] + E),
+    "minicpmo_gpu_context_qwen3_sample_batch": (i32, [vp, sz, fptr, i32ptr, fptr, fptr, fptr, u32ptr, fptr, i32ptr] + E),
     "minicpmo_gpu_context_qwen3_time_decode_batch": (i32, [vp, sz, u32ptr, u32ptr, sz, fptr] + E),
     "minicpmo_gpu_context_qwen3_batch_kernels": (i32, [vp, i32]),
     "minicpmo_gpu_context_time_matvec": (i32, [vp, vp, sz, sz, i32, fptr] + E),
@@ -540,6 +541,22 @@ class GpuContext:
         self._call("minicpmo_gpu_context_qwen3_decode_batch", t.size, t.ctypes.data_as(u32ptr), p.ctypes.data_as(u32ptr),
                    n_steps, out.ctypes.data_as(u32ptr))
         return out
+
+    def qwen3_sample_batch(self, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
+        """One token per sequence from the last batched step's logits: (tokens, probabilities, kept counts).
+        Parameters are one value for all sequences or one each; None for off."""
+        u = _as_f32(uniform).reshape(-1)
+        n = u.size
+
+        def each(v, dtype):
+            return None if v is None else np.ascontiguousarray(np.broadcast_to(np.asarray(v, dtype), (n,)))
+
+        t, p, m, k = each(temperature, np.float32), each(top_p, np.float32), each(min_p, np.float32), each(top_k, np.int32)
+        tokens, probs, kept = np.zeros(n, np.uint32), np.zeros(n, np.float32), np.zeros(n, np.int32)
+        f = lambda a: None if a is None else _f(a)  # noqa: E731
+        self._call("minicpmo_gpu_context_qwen3_sample_batch", n, f(t), None if k is None else k.ctypes.data_as(i32ptr), f(p),
+                   f(m), _f(u), tokens.ctypes.data_as(u32ptr), _f(probs), kept.ctypes.data_as(i32ptr))
+        return tokens, probs, kept
 
     def qwen3_time_decode_batch(self, first_tokens, first_positions, n_steps: int) -> float:
         t = np.ascontiguousarray(first_tokens, dtype=np.uint32)

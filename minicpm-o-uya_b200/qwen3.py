@@ -211,6 +211,28 @@ class Qwen3Runtime:
         self.batch_last = toks[:, -1].copy()
         return out
 
+    def sample_batch(self, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
+        """Draw every sequence's next token from the last step's logits with the given uniform random numbers:
+        (tokens, probabilities, kept counts).  Parameters: one value, one per sequence, or None for off."""
+        return self.gpu.qwen3_sample_batch(uniform, temperature, top_k, top_p, min_p)
+
+    def generate_batch_sampled(self, n_new: int, uniform, temperature=None, top_k=None, top_p=None,
+                               min_p=None) -> np.ndarray:
+        """Sampled decode of every sequence after append_prompt_batch: tokens [n_seq][n], each drawn from the logits
+        behind the one before it with uniform[i][n_seq]; all of them are forwarded, so that sampling, or generate_batch
+        from the greedy choice, goes on behind them."""
+        start = self.batch_tokens
+        n = min(n_new, self.context - start)
+        u = np.asarray(uniform, np.float32).reshape(-1, len(self.batch_last))
+        if u.shape[0] < n:
+            raise ValueError(f"error: {u.shape[0]} rows of random numbers for {n} tokens")
+        out = np.zeros((len(self.batch_last), max(n, 0)), np.uint32)
+        for i in range(n):
+            out[:, i], _, _ = self.sample_batch(u[i], temperature, top_k, top_p, min_p)
+            self.batch_last, _, _ = self.forward_batch(out[:, i], np.full(out.shape[0], start + i, np.uint32))
+            self.batch_tokens = start + i + 1
+        return out
+
     def generate_device(self, n_new: int, penalty: float = 1.0) -> List[int]:
         """Greedy decode with the sampled token fed back on the device (no host round trip per token)."""
         n = min(n_new, self.context - self.total_tokens)
