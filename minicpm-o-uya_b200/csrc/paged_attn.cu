@@ -52,23 +52,27 @@ __device__ __forceinline__ bool paged_last(const PagedAttnArgs& a, const PagedPi
 // ---------------------------------------------------------------------
 // f32: FMAs
 // ---------------------------------------------------------------------
-// f32 products keep f32's accuracy only on the FMA units.  A block is 16 rows;
-// a thread has two rows x two keys of the scores and two rows x head_dim / 16
-// columns of the output, so shared memory gives each operand to 16 threads.
-// Shared-memory reads bound it (6 wavefronts per 16 FMAs of a warp), about
-// half of the FMA rate.  A warp copies 8 keys of a tile: one table entry each.
+// f32 products keep f32's accuracy on the FMA units; split into tf32 or bf16
+// parts for the matrix units they took longer (three m16n8k8 tf32 products per
+// step: 126 us where this takes less than half).  What bounds an FMA kernel is
+// shared-memory reads, so threads take 4 x 4 tiles: for the scores a warp has
+// all 16 rows x 32 keys over a quarter of head_dim (8 reads of 16 bytes per 64
+// FMAs; the four warps' sums are added on the way to the softmax), for the
+// output all rows x a quarter of the columns (2 reads per 16 FMAs).  Rows and
+// keys are dealt out so that a warp's reads meet all banks.
 constexpr int kSimtRows = 16, kSimtKeys = 32, kSimtThreads = 128;
 
 template <int HD>
 struct SimtSmem {
-  float q[kSimtRows][HD];
+  float q[kSimtRows][HD + 4];
   float k[2][kSimtKeys][HD + 4];
   float v[2][kSimtKeys][HD];
-  float p[kSimtRows][kSimtKeys];
+  float part[4][kSimtRows][kSimtKeys + 8];  // scores over a warp's part of head_dim
+  float p[kSimtRows][kSimtKeys + 4];
+  float corr[kSimtRows], m[kSimtRows], l[kSimtRows];
 };
-
 template <int HD>
-constexpr int kSimtCtas = HD == 64 ? 4 : HD == 128 ? 3 : 1;  // per SM, by shared memory and registers
+constexpr int kSimtCtas = HD == 64 ? 4 : HD == 128 ? 2 : 1;  // per SM, by shared memory
 
 template <int HD>
 __global__ void __launch_bounds__(kSimtThreads, kSimtCtas<HD>) k_paged_attn_f32(const PagedAttnArgs a) {
@@ -76,15 +80,16 @@ __global__ void __launch_bounds__(kSimtThreads, kSimtCtas<HD>) k_paged_attn_f32(
   SimtSmem<HD>& s = *reinterpret_cast<SimtSmem<HD>*>(smem_raw);
   __shared__ PagedShared sched;
   __shared__ unsigned last_s;
-  constexpr int kCols = HD / 16;  // accumulator columns of a thread, for each of its two rows
-  const int tid = threadIdx.x, x = tid & 15, y = tid >> 4;  // rows 2y, 2y + 1
-  const int warp = tid >> 5, lane = tid & 31;
+  constexpr int kC = HD / 32;  // output columns of a thread, for each of its four rows
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rg = lane >> 3, kl = lane & 7;
+  const int col = warp * (HD / 4) + kl * kC;  // rows 4 i + rg, i < 4
+  const int srow = tid >> 3, skey = (tid & 7) * 4;  // in the softmax: a row, four keys
   const int block_tokens = kSimtRows / a.group;
   const float* qg = static_cast<const float*>(a.q);
   const float* kg = static_cast<const float*>(a.kc);
   const float* vg = static_cast<const float*>(a.vc);
   PagedWalk<kSimtKeys> walk;
-  walk.start(a, &sched, block_tokens, 0);
+  walk.start(a, &sched, block_tokens, 0, 3);
   PagedPiece p;
   while (walk.next(a, &p)) {
     const int t0 = p.b * block_tokens, rows = min(block_tokens, p.req.n_new - t0) * a.group;
@@ -117,157 +122,196 @@ __global__ void __launch_bounds__(kSimtThreads, kSimtCtas<HD>) k_paged_attn_f32(
                                              (long long)(p.h * a.group + row % a.group) * HD + c);
       *reinterpret_cast<float4*>(&s.q[row][c]) = v;
     }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[2][kCols];
-    int see[2];  // keys that each row sees (rows without a token: all, so that they mask nothing)
+    // keys that a row sees (rows without a token: all, so that they mask nothing)
+    auto sees = [&](int row) {
+      return row < rows ? max(0, p.req.len - p.req.n_new + t0 + row / a.group + 1) : INT_MAX;
+    };
+    const int see_s = sees(srow), see_all = max(0, p.req.len - p.req.n_new + t0 + 1);
+    const int see[4] = {sees(rg), sees(4 + rg), sees(8 + rg), sees(12 + rg)};
+    float m = -INFINITY, l = 0.f, acc[4][kC];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = 2 * y + i;
-      see[i] = row < rows ? max(0, p.req.len - p.req.n_new + t0 + row / a.group + 1) : INT_MAX;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) acc[i][c] = 0.f;
-    }
+      for (int c = 0; c < kC; ++c) acc[i][c] = 0.f;
     for (int tile = p.tile0; tile < p.tile1; ++tile) {
       const int st = (tile - p.tile0) & 1, key0 = tile * kSimtKeys;
+      cp_async_wait<0>();
+      __syncthreads();  // this tile is there, and everyone is done with the last one
       if (tile + 1 < p.tile1) {
         load(tile + 1, st ^ 1, next_page);
         next_page = page(tile + 2);
-        cp_async_wait<1>();
-      } else {
-        cp_async_wait<0>();
+      }
+      float sc[4][4] = {};
+#pragma unroll 2
+      for (int d = warp * (HD / 4); d < (warp + 1) * (HD / 4); d += 4) {
+        float4 q4[4], k4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          q4[i] = *reinterpret_cast<const float4*>(&s.q[4 * i + rg][d]);
+          k4[i] = *reinterpret_cast<const float4*>(&s.k[st][8 * i + kl][d]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[i][j] = fmaf(q4[i].x, k4[j].x, sc[i][j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[i][j] = fmaf(q4[i].y, k4[j].y, sc[i][j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[i][j] = fmaf(q4[i].z, k4[j].z, sc[i][j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[i][j] = fmaf(q4[i].w, k4[j].w, sc[i][j]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s.part[warp][4 * i + rg][8 * j + kl] = sc[i][j];
+      __syncthreads();
+      {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 y = *reinterpret_cast<const float4*>(&s.part[w][srow][skey]);
+          x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+        }
+        const int left = see_s - key0 - skey;  // of the four keys, those that the row sees
+        x.x = left > 0 ? x.x * a.scale_log2 : -INFINITY;
+        x.y = left > 1 ? x.y * a.scale_log2 : -INFINITY;
+        x.z = left > 2 ? x.z * a.scale_log2 : -INFINITY;
+        x.w = left > 3 ? x.w * a.scale_log2 : -INFINITY;
+        float mx = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - base);
+        m = mn;
+        x = make_float4(exp2f(x.x - base), exp2f(x.y - base), exp2f(x.z - base), exp2f(x.w - base));
+        float sum = (x.x + x.y) + (x.z + x.w);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        l = l * corr + sum;
+        *reinterpret_cast<float4*>(&s.p[srow][skey]) = x;
+        if ((tid & 7) == 0) s.corr[srow] = corr;
       }
       __syncthreads();
-      float sc[2][2] = {};
-#pragma unroll 4
-      for (int d = 0; d < HD; d += 4) {
-        const float4 q0 = *reinterpret_cast<const float4*>(&s.q[2 * y][d]);
-        const float4 q1 = *reinterpret_cast<const float4*>(&s.q[2 * y + 1][d]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float4 k4 = *reinterpret_cast<const float4*>(&s.k[st][x + 16 * j][d]);
-          sc[0][j] = fmaf(q0.x, k4.x, fmaf(q0.y, k4.y, fmaf(q0.z, k4.z, fmaf(q0.w, k4.w, sc[0][j]))));
-          sc[1][j] = fmaf(q1.x, k4.x, fmaf(q1.y, k4.y, fmaf(q1.z, k4.z, fmaf(q1.w, k4.w, sc[1][j]))));
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float f = s.corr[4 * i + rg];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) acc[i][c] *= f;
       }
+      auto value = [&](int key, float (&v)[kC]) {
+        const float* at = &s.v[st][key][col];
+        if constexpr (kC == 2) {
+          const float2 x = *reinterpret_cast<const float2*>(at);
+          v[0] = x.x, v[1] = x.y;
+        } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          sc[i][j] = key0 + x + 16 * j < see[i] ? sc[i][j] * a.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, sc[i][j]);
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn;
-        const float corr = exp2f(m[i] - base);
-        m[i] = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float w = exp2f(sc[i][j] - base);
-          sum += w;
-          s.p[2 * y + i][x + 16 * j] = w;
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        l[i] = l[i] * corr + sum;
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) acc[i][c] *= corr;
-      }
-      __syncwarp();
-      auto add = [&](int key, float w0, float w1, bool on0, bool on1) {
-#pragma unroll
-        for (int c = 0; c < kCols; c += 4) {
-          const float4 v4 = *reinterpret_cast<const float4*>(&s.v[st][key][x * 4 + c * 16]);
-          if (on0) {
-            acc[0][c] = fmaf(w0, v4.x, acc[0][c]);
-            acc[0][c + 1] = fmaf(w0, v4.y, acc[0][c + 1]);
-            acc[0][c + 2] = fmaf(w0, v4.z, acc[0][c + 2]);
-            acc[0][c + 3] = fmaf(w0, v4.w, acc[0][c + 3]);
-          }
-          if (on1) {
-            acc[1][c] = fmaf(w1, v4.x, acc[1][c]);
-            acc[1][c + 1] = fmaf(w1, v4.y, acc[1][c + 1]);
-            acc[1][c + 2] = fmaf(w1, v4.z, acc[1][c + 2]);
-            acc[1][c + 3] = fmaf(w1, v4.w, acc[1][c + 3]);
+          for (int c = 0; c < kC; c += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(at + c);
+            v[c] = x.x, v[c + 1] = x.y, v[c + 2] = x.z, v[c + 3] = x.w;
           }
         }
       };
-      const bool all = key0 + kSimtKeys <= see[0] && key0 + kSimtKeys <= see[1];
-      if (__all_sync(0xffffffffu, all)) {
+      if (key0 + kSimtKeys <= see_all) {
 #pragma unroll 2
         for (int key = 0; key < kSimtKeys; key += 4) {
-          const float4 w0 = *reinterpret_cast<const float4*>(&s.p[2 * y][key]);
-          const float4 w1 = *reinterpret_cast<const float4*>(&s.p[2 * y + 1][key]);
-          add(key, w0.x, w1.x, true, true);
-          add(key + 1, w0.y, w1.y, true, true);
-          add(key + 2, w0.z, w1.z, true, true);
-          add(key + 3, w0.w, w1.w, true, true);
-        }
-      } else {
-        // a key that a row does not see adds nothing, whatever V holds there
-#pragma unroll 1
-        for (int key = 0; key < kSimtKeys; ++key)
-          add(key, s.p[2 * y][key], s.p[2 * y + 1][key], key0 + key < see[0], key0 + key < see[1]);
-      }
-      __syncthreads();
-    }
-    bool write = p.n_ctas == 1;
-    if (!write) {
-      float* part = a.partial + paged_slot(blockIdx.x, p.first_cta) * kSimtRows * (HD + 4);
+          float4 w[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float* row = part + (2 * y + i) * (HD + 4);
+          for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4*>(&s.p[4 * i + rg][key]);
 #pragma unroll
-        for (int c = 0; c < kCols; c += 4)
-          *reinterpret_cast<float4*>(row + 4 + x * 4 + c * 16) =
-              make_float4(acc[i][c], acc[i][c + 1], acc[i][c + 2], acc[i][c + 3]);
-        if (x == 0) row[0] = m[i], row[1] = l[i];
-      }
-      if (paged_last(a, p, &last_s)) {
-        write = true;
+          for (int j = 0; j < 4; ++j) {
+            float v[kC];
+            value(key + j, v);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          m[i] = -INFINITY, l[i] = 0.f;
-          for (int c = 0; c < p.n_ctas; ++c)
-            m[i] = fmaxf(m[i], __ldcg(a.partial + paged_slot(p.first_cta + c, p.first_cta) * kSimtRows * (HD + 4) +
-                                      (2 * y + i) * (HD + 4)));
-          const float base = m[i] == -INFINITY ? 0.f : m[i];
+            for (int i = 0; i < 4; ++i) {
+              const float x = j == 0 ? w[i].x : j == 1 ? w[i].y : j == 2 ? w[i].z : w[i].w;
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) acc[i][c] = 0.f;
-          for (int c = 0; c < p.n_ctas; ++c) {
-            const float* row = a.partial + paged_slot(p.first_cta + c, p.first_cta) * kSimtRows * (HD + 4) +
-                               (2 * y + i) * (HD + 4);
-            const float f = exp2f(__ldcg(row) - base);
-            l[i] += __ldcg(row + 1) * f;
-#pragma unroll
-            for (int cc = 0; cc < kCols; cc += 4) {
-              const float4 v4 = __ldcg(reinterpret_cast<const float4*>(row + 4 + x * 4 + cc * 16));
-              acc[i][cc] += v4.x * f;
-              acc[i][cc + 1] += v4.y * f;
-              acc[i][cc + 2] += v4.z * f;
-              acc[i][cc + 3] += v4.w * f;
+              for (int c = 0; c < kC; ++c) acc[i][c] = fmaf(x, v[c], acc[i][c]);
             }
           }
         }
+      } else {
+        // a key that a row does not see adds nothing, whatever V holds there
+#pragma unroll 4
+        for (int key = 0; key < kSimtKeys; ++key) {
+          float v[kC];
+          value(key, v);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = s.p[4 * i + rg][key];
+            const bool on = key0 + key < see[i];
+#pragma unroll
+            for (int c = 0; c < kC; ++c) acc[i][c] = on ? fmaf(x, v[c], acc[i][c]) : acc[i][c];
+          }
+        }
+      }
+    }
+    if ((tid & 7) == 0) s.m[srow] = m, s.l[srow] = l;
+    __syncthreads();
+    float rm[4], rl[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rm[i] = s.m[4 * i + rg], rl[i] = s.l[4 * i + rg];
+    bool write = p.n_ctas == 1;
+    constexpr int kLd = HD + 4;
+    if (!write) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float* row = a.partial + (paged_slot(blockIdx.x, p.first_cta) * kSimtRows + 4 * i + rg) * kLd;
+#pragma unroll
+        for (int c = 0; c < kC; c += 2) *reinterpret_cast<float2*>(row + 4 + col + c) = make_float2(acc[i][c], acc[i][c + 1]);
+        if (warp == 0 && kl == 0) *reinterpret_cast<float2*>(row) = make_float2(rm[i], rl[i]);
+      }
+      if (paged_last(a, p, &last_s)) {
+        write = true;
+        const float* row0 = a.partial + rg * kLd;
+        auto at = [&](int k, int i) {
+          return row0 + (paged_slot(p.first_cta + k, p.first_cta) * kSimtRows + 4 * i) * kLd;
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          rm[i] = -INFINITY, rl[i] = 0.f;
+#pragma unroll
+          for (int c = 0; c < kC; ++c) acc[i][c] = 0.f;
+        }
+#pragma unroll 4
+        for (int k = 0; k < p.n_ctas; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rm[i] = fmaxf(rm[i], __ldcg(at(k, i)));
+#pragma unroll 2
+        for (int k = 0; k < p.n_ctas; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(at(k, i)));
+            const float f = exp2f(ml.x - (rm[i] == -INFINITY ? 0.f : rm[i]));
+            rl[i] += ml.y * f;
+#pragma unroll
+            for (int c = 0; c < kC; c += 2) {
+              const float2 v = __ldcg(reinterpret_cast<const float2*>(at(k, i) + 4 + col + c));
+              acc[i][c] += v.x * f, acc[i][c + 1] += v.y * f;
+            }
+          }
       }
     }
     if (write) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = 2 * y + i;
+      for (int i = 0; i < 4; ++i) {
+        const int row = 4 * i + rg;
         if (row >= rows) continue;
         const long long t = p.req.q0 + t0 + row / a.group;
         const int head = p.h * a.group + row % a.group;
-        const float inv = see[i] > 0 ? 1.0f / l[i] : 0.f;
-        float* o = static_cast<float*>(a.out) + t * a.out_stride + (long long)head * HD;
+        const bool any = see[i] > 0;
+        const float inv = any ? 1.0f / rl[i] : 0.f;
+        float* o = static_cast<float*>(a.out) + t * a.out_stride + (long long)head * HD + col;
 #pragma unroll
-        for (int c = 0; c < kCols; c += 4)
-          *reinterpret_cast<float4*>(o + x * 4 + c * 16) =
-              see[i] > 0 ? make_float4(acc[i][c] * inv, acc[i][c + 1] * inv, acc[i][c + 2] * inv, acc[i][c + 3] * inv)
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
-        if (a.lse && x == 0)
-          a.lse[t * a.q_heads + head] = see[i] > 0 ? 0.693147180559945309f * (m[i] + log2f(l[i])) : -INFINITY;
+        for (int c = 0; c < kC; c += 2)
+          *reinterpret_cast<float2*>(o + c) = any ? make_float2(acc[i][c] * inv, acc[i][c + 1] * inv) : make_float2(0.f, 0.f);
+        if (a.lse && warp == 0 && kl == 0)
+          a.lse[t * a.q_heads + head] = any ? 0.693147180559945309f * (rm[i] + log2f(rl[i])) : -INFINITY;
       }
     }
     __syncthreads();  // the next piece's loads overwrite the tiles
@@ -320,7 +364,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<HD>::kCtas) k_paged_attn_m
   const uint32_t ring_a = smem_addr(ring);
   const int block_tokens = kMmaRows / a.group;
   PagedWalk<kMmaTile> walk;
-  walk.start(a, &sched, block_tokens, 0);
+  walk.start(a, &sched, block_tokens, 0, 1);
   PagedPiece p;
   while (walk.next(a, &p)) {
     const int t0 = p.b * block_tokens, rows = min(block_tokens, p.req.n_new - t0) * a.group;

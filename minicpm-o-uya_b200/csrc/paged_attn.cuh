@@ -144,7 +144,7 @@ struct PagedWalk {
   }
 
   // Block-wide: every thread of the CTA calls it, and gets the same walk.
-  __device__ __forceinline__ void start(const PagedAttnArgs& a, PagedShared* s, int block_tokens_, int snap_) {
+  __device__ __forceinline__ void start(const PagedAttnArgs& a, PagedShared* s, int block_tokens_, int snap_, int min_units) {
     block_tokens = block_tokens_;
     snap = snap_;
     const int n = a.n_req, nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -167,9 +167,10 @@ struct PagedWalk {
     }
     const long long ex = base + incl - mine;
     total = all;
-    ctas = (int)min((long long)gridDim.x, total);
+    // a CTA with less than min_units would cost its piece's join more than it saves
+    ctas = (int)min((long long)gridDim.x, max(1ll, total / min_units));
     u = u1 = total;
-    if ((int)blockIdx.x >= ctas) return;  // the same for the whole block
+    if ((int)blockIdx.x >= ctas || total == 0) return;  // the same for the whole block
     const long long x0 = (long long)blockIdx.x * total / ctas, x1 = (long long)(blockIdx.x + 1) * total / ctas;
     if (x1 < total) {
       locate(a, s, x1, ex, mine, r0, r1);

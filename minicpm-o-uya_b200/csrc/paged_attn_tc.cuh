@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __shared__ PagedPiece pieces[kTcThreads / 32];
   {
     PagedWalk<kTcKeys> walk;
-    walk.start(a, &sched, block_tokens, 4);  // has barriers: the inits above are seen behind them
+    walk.start(a, &sched, block_tokens, 4, 1);  // has barriers: the inits above are seen behind them
     if (lane == 0) walks[warp] = walk;
   }
   tc_fence_before();
