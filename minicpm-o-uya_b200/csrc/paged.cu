@@ -483,7 +483,7 @@ int minicpmo_gpu_paged_plan(const int32_t* lens, const int32_t* new_lens, size_t
     attr[0].val.clusterDim.x = (unsigned)ctas;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = ctas > 1 ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, k_paged_plan, a);
   }
   if (e != cudaSuccess) return paged_error(error, error_cap, "error: %s: launch: %s", op, cudaGetErrorString(e));

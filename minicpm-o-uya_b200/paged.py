@@ -29,6 +29,7 @@ MAX_REQUESTS = 8192  # MINICPMO_PAGED_MAX_REQUESTS
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 _local = threading.local()  # this thread's error buffer
+_entry: dict = {}  # the library's entry points by name
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -42,7 +43,9 @@ def _call(name: str, index: int, *args) -> None:
         err = _local.err
     except AttributeError:
         err = _local.err = C.create_string_buffer(ERR_CAP)
-    fn = getattr(lib(), name)
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(lib(), name)
     if torch._C._cuda_getDevice() == index:
         ok = fn(*args, torch._C._cuda_getCurrentRawStream(index), err, ERR_CAP)
     else:
