@@ -531,12 +531,16 @@ MINICPMO_API int minicpmo_gpu_paged_append(const minicpmo_paged_cache *cache, co
  * heads contiguous, tokens q_stride / out_stride elements apart; rows at
  * cu_new[n_req] and behind it are left as they are.  q_heads is a multiple of
  * kv_heads, at most 16 per kv head.  Table entries outside the cache read as
- * rows of zeros.  Scores, softmax statistics and sums are f32; for F16 and
+ * rows of zeros; lens is clamped to what a table row holds (max_pages *
+ * page_size, at most 2^30).  Scores, softmax statistics and sums are f32; for F16 and
  * BF16 the softmax weights are rounded to the cache's type for the product
  * with V.  workspace: MINICPMO_PAGED_WORKSPACE_BYTES, zero before its first
  * use, 256-byte aligned; each call leaves it ready for the next.  Calls that
  * may overlap on the GPU (streams, graphs replayed side by side) need one
- * each. */
+ * each.  A bounded wait inside a kernel that gives up (only a fault elsewhere
+ * on the device makes one) sets the int at byte 4096 of the workspace, which
+ * is not reported back: that call's output is undefined, and the workspace has
+ * to be cleared. */
 MINICPMO_API int minicpmo_gpu_paged_attention(const minicpmo_paged_cache *cache, const void *q, size_t n_tokens,
                                  size_t q_heads, size_t q_stride, const int32_t *block_table, size_t max_pages,
                                  size_t table_stride, const int32_t *lens, const int32_t *cu_new, size_t n_req,

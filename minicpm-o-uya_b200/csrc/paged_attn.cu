@@ -769,7 +769,7 @@ extern "C" int minicpmo_gpu_paged_attention(const minicpmo_paged_cache* cache, c
     return paged_error(error, error_cap, "error: %s: %zu q heads over %zu kv heads (need a multiple, at most %d each)",
                        op, q_heads, kv, kPagedMaxGroup);
   if (n_tokens > (1u << 24)) return paged_error(error, error_cap, "error: %s: %zu tokens", op, n_tokens);
-  if (max_pages < 1 || max_pages > (size_t)INT_MAX / cache->page_size || table_stride < max_pages ||
+  if (max_pages < 1 || max_pages > (size_t)(1 << 30) / cache->page_size || table_stride < max_pages ||
       table_stride > (1ull << 40))
     return paged_error(error, error_cap, "error: %s: table rows of %zu pages, %zu apart", op, max_pages, table_stride);
   if (q_stride < q_heads * hd || out_stride < q_heads * hd || q_stride > (1ull << 40) || out_stride > (1ull << 40))

@@ -526,3 +526,55 @@ def test_negative_scale_and_one_workspace_for_many_shapes(pkg):
         c = _attention_case(seed, dtype, hd, heads, kv, page, reqs)
         for scale in (-0.05, 0.0, 0.11):
             _check_attention(c, *_run_attention(paged, c, ws, scale), scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd, heads, kv, page, reqs", [
+    (128, 8, 2, 8, [(0, 70), (3, 90), (200, 150), (0, 0), (64, 64)]),  # tokens before the cache's beginning see nothing
+    (128, 16, 1, 256, [(900, 130), (257, 257)]), (64, 3, 3, 32, [(129, 128), (500, 129), (128, 1)]),
+    (128, 7, 1, 16, [(333, 300), (20, 19)]), (64, 16, 1, 64, [(65, 65)] * 7), (128, 10, 2, 128, [(1000, 513), (4, 4), (700, 1)]),
+    (128, 32, 8, 64, [(2500, 600), (1, 1), (3000, 40), (90, 90)]),
+])
+def test_attention_of_long_chunks(pkg, dtype, hd, heads, kv, page, reqs):
+    """Many rows per request: the 256-row blocks, both tiles of them or one, every group size and page size."""
+    from minicpmo_b200 import paged
+
+    c = _attention_case(31, dtype, hd, heads, kv, page, reqs, heads_out=page == 16)
+    ws = paged.workspace()
+    first = _run_attention(paged, c, ws)
+    _check_attention(c, *first)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, _run_attention(paged, c, ws)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n_req, chunk", [(1000, 1), (8192, 1), (700, 9)])
+def test_attention_of_many_requests(pkg, dtype, n_req, chunk):
+    from minicpmo_b200 import paged
+
+    rng = np.random.default_rng(n_req)
+    reqs = [(int(n), int(min(n, rng.integers(0, chunk + 1)))) for n in rng.integers(0, 40, n_req)]
+    c = _attention_case(5, dtype, 64, 8 if chunk > 1 else 2, 1, 16, reqs, spoil=False)
+    _check_attention(c, *_run_attention(paged, c, paged.workspace()))
+
+
+@pytest.mark.gpu
+def test_workspaces_apart_on_two_streams(pkg):
+    """Two calls that overlap, each with its own workspace, give what they give alone."""
+    from minicpmo_b200 import paged
+
+    a = _attention_case(1, "bf16", 128, 32, 8, 16, [(4000, 1)] * 8)
+    b = _attention_case(2, "bf16", 128, 32, 8, 64, [(1200, 600)] * 2)
+    wa, wb = paged.workspace(), paged.workspace()
+    alone = [_run_attention(paged, a, wa), _run_attention(paged, b, wb)]
+    torch.cuda.synchronize()
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(20):
+        with torch.cuda.stream(sa):
+            ra = _run_attention(paged, a, wa)
+        with torch.cuda.stream(sb):
+            rb = _run_attention(paged, b, wb)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for r, s in zip((ra, rb), alone) for x, y in zip(r, s))
