@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kSimtThreads, kSimtCtas<HD>) k_paged_attn_f32(
   const float* kg = static_cast<const float*>(a.kc);
   const float* vg = static_cast<const float*>(a.vc);
   PagedWalk<kSimtKeys> walk;
-  walk.start(a, &sched, block_tokens, 0, 3);
+  walk.start(a, &sched, block_tokens, 0, 3, 0.f);  // a unit takes long next to a join here: 1 instead of 0 made 16,000 keys 40% slower
   PagedPiece p;
   while (walk.next(a, &p)) {
     const int t0 = p.b * block_tokens, rows = min(block_tokens, p.req.n_new - t0) * a.group;
@@ -366,7 +366,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<HD>::kCtas) k_paged_attn_m
   const uint32_t ring_a = smem_addr(ring);
   const int block_tokens = kMmaRows / a.group;
   PagedWalk<kMmaTile> walk;
-  walk.start(a, &sched, block_tokens, 0, 1);
+  // join_units: one request of 4,000 keys takes 25.3, 19.5 and 21.9 us at 0, 1/4 and 1
+  walk.start(a, &sched, block_tokens, 0, 1, 0.3f);
   PagedPiece p;
   while (walk.next(a, &p)) {
     const int t0 = p.b * block_tokens, rows = min(block_tokens, p.req.n_new - t0) * a.group;
@@ -591,12 +592,13 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<HD>::kCtas) k_paged_attn_m
         write = true;
         if (row < rows) {
           mm = -INFINITY, ll = 0.f;
+#pragma unroll 8
           for (int c = 0; c < p.n_ctas; ++c)
             mm = fmaxf(mm, __ldcg(a.partial + (paged_slot(p.first_cta + c, p.first_cta) * kMmaRows + row) * kLd));
           const float b = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
           for (int c = 0; c < HD / 32; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+#pragma unroll(HD == 256 ? 2 : 4)
           for (int k = 0; k < p.n_ctas; ++k) {
             const float* src = a.partial + (paged_slot(p.first_cta + k, p.first_cta) * kMmaRows + row) * kLd;
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(src));
@@ -731,8 +733,13 @@ cudaError_t launch_tc(const PagedAttnArgs& a, const TcMaps& m, cudaStream_t st) 
 template <typename T>
 cudaError_t launch_16(const PagedAttnArgs& a, int hd, cudaStream_t st) {
   // Many rows per request: 256-row blocks on the tensor cores.  Few: 16-row
-  // blocks, whose time is the K/V stream's.
-  if (hd <= 128 && a.scale_log2 > 0.f && (long long)a.n_tokens * a.group >= 64ll * a.n_req) {
+  // blocks, whose time is the K/V stream's.  Behind 4,000 keys (8 K/V heads of
+  // 128, bf16), 16-row against 256-row blocks: 32 requests of 21 rows 88 and
+  // 118 us, of 42 147 and 118; 8 of 22 41 and 49, of 45 57 and 50; one request
+  // has few blocks to share the SMs out to, and a join: 128 rows 35 and 45, 256
+  // 52 and 47.
+  if (hd <= 128 && a.scale_log2 > 0.f && (long long)a.n_tokens * a.group >= 40ll * a.n_req &&
+      (long long)a.n_tokens * a.q_heads >= 1536) {
     TcMaps m;
     if (tc_maps(&m, a, hd, Frag<T>::kExp == 0x7f807f80u))
       return hd == 64 ? launch_tc<T, 64>(a, m, st) : launch_tc<T, 128>(a, m, st);

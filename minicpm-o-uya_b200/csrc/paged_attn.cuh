@@ -75,6 +75,7 @@ __device__ __forceinline__ long long paged_head_units(const PagedReq& q, int blo
 
 struct PagedShared {
   long long red[32];
+  int longest[32];
   long long total, before;  // all units; those before request r
   int r;                    // the request of this CTA's first unit
 };
@@ -144,13 +145,20 @@ struct PagedWalk {
   }
 
   // Block-wide: every thread of the CTA calls it, and gets the same walk.
-  __device__ __forceinline__ void start(const PagedAttnArgs& a, PagedShared* s, int block_tokens_, int snap_, int min_units) {
+  __device__ __forceinline__ void start(const PagedAttnArgs& a, PagedShared* s, int block_tokens_, int snap_, int min_units,
+                                        float join_units) {
     block_tokens = block_tokens_;
     snap = snap_;
     const int n = a.n_req, nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (n + nt - 1) / nt, r0 = min(n, tid * per), r1 = min(n, r0 + per);
     long long mine = 0;
-    for (int i = r0; i < r1; ++i) mine += paged_head_units<KT>(paged_req(a, i, block_tokens), block_tokens);
+    int longest = 0;  // units of the longest block
+    for (int i = r0; i < r1; ++i) {
+      const PagedReq q = paged_req(a, i, block_tokens);
+      mine += paged_head_units<KT>(q, block_tokens);
+      if (q.blocks > 0) longest = max(longest, paged_tiles<KT>(q, q.blocks - 1, block_tokens));
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
     mine *= a.kv_heads;
     long long incl = mine;
 #pragma unroll
@@ -158,17 +166,22 @@ struct PagedWalk {
       const long long v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    if (lane == 31) s->red[warp] = incl;
+    if (lane == 31) s->red[warp] = incl, s->longest[warp] = longest;
     __syncthreads();
     long long base = 0, all = 0;
     for (int w = 0; w < nt / 32; ++w) {
       if (w < warp) base += s->red[w];
       all += s->red[w];
+      longest = max(longest, s->longest[w]);
     }
     const long long ex = base + incl - mine;
     total = all;
-    // a CTA with less than min_units would cost its piece's join more than it saves
-    ctas = (int)min((long long)gridDim.x, max(1ll, total / min_units));
+    // Pieces of c units make the longest block of n take about c for its own
+    // piece and join_units * n / c for the join, one piece behind the other:
+    // least at c = sqrt(join_units * n), and no CTA takes less than that while
+    // there are more CTAs than the units need.
+    const int least = max(min_units, (int)sqrtf(join_units * (float)longest));
+    ctas = (int)min((long long)gridDim.x, max(1ll, total / least));
     u = u1 = total;
     if ((int)blockIdx.x >= ctas || total == 0) return;  // the same for the whole block
     const long long x0 = (long long)blockIdx.x * total / ctas, x1 = (long long)(blockIdx.x + 1) * total / ctas;

@@ -323,7 +323,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __shared__ PagedPiece pieces[kTcThreads / 32];
   {
     PagedWalk<kTcKeys> walk;
-    walk.start(a, &sched, block_tokens, 4, 1);  // has barriers: the inits above are seen behind them
+    // join_units: 64 tokens behind 4,000 take 64, 55 and 43 us at 0, 1/4 and 1,
+    // 512 behind 200 18.2, 18.0 and 22.7.
+    walk.start(a, &sched, block_tokens, 4, 1, 0.5f);  // has barriers: the inits above are seen behind them
     if (lane == 0) walks[warp] = walk;
   }
   tc_fence_before();
@@ -592,8 +594,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool wild = s.wild != 0 && p.tile1 * kTcKeys > see_all;
       const long long tok_g = p.req.q0 + tok;
       const int head = p.h * a.group + row % a.group;
-      float* part = a.partial + (paged_slot(blockIdx.x, p.first_cta) * 256 + t * 128 + row) * kLd;
+      // A piece's O is stored by fours of columns, the rows of each next to one
+      // another: a warp's 32 threads, one row each, store and load 512 bytes in
+      // a row.  (With the rows of O end to end a store took 8,700 cycles and a
+      // join of 17 pieces 135,000; these take 3,800 and 61,000.)
+      float* const part0 = a.partial + t * 128 * kLd;
+      const long long slot_f = 256ll * kLd;
+      float* part = part0 + paged_slot(blockIdx.x, p.first_cta) * slot_f;
       T* dst = static_cast<T*>(a.out) + tok_g * a.out_stride + (long long)head * HD;
+      auto store = [&](int c, const float (&o)[32], float inv) {  // 32 columns of out
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) {
+          uint4 u;
+          u.x = Frag<T>::pack(o[k] * inv, o[k + 1] * inv);
+          u.y = Frag<T>::pack(o[k + 2] * inv, o[k + 3] * inv);
+          u.z = Frag<T>::pack(o[k + 4] * inv, o[k + 5] * inv);
+          u.w = Frag<T>::pack(o[k + 6] * inv, o[k + 7] * inv);
+          *reinterpret_cast<uint4*>(dst + c + k) = u;
+        }
+      };
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         float o[32];
@@ -621,24 +640,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
         if (whole) {
-#pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            uint4 u;
-            u.x = Frag<T>::pack(o[k] * inv, o[k + 1] * inv);
-            u.y = Frag<T>::pack(o[k + 2] * inv, o[k + 3] * inv);
-            u.z = Frag<T>::pack(o[k + 4] * inv, o[k + 5] * inv);
-            u.w = Frag<T>::pack(o[k + 6] * inv, o[k + 7] * inv);
-            *reinterpret_cast<uint4*>(dst + c + k) = u;
-          }
+          store(c, o, inv);
         } else {
 #pragma unroll
           for (int k = 0; k < 32; k += 4)
-            *reinterpret_cast<float4*>(part + 4 + c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            *reinterpret_cast<float4*>(part + ((c + k) / 4 * 128 + row) * 4) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
       }
       if (valid && whole && a.lse)
         a.lse[tok_g * a.q_heads + head] = see > 0 ? 0.693147180559945309f * (m + log2f(l)) : -INFINITY;
-      if (valid && !whole) *reinterpret_cast<float2*>(part) = make_float2(m, l);
+      if (valid && !whole) *reinterpret_cast<float2*>(part + 128 * HD + 2 * row) = make_float2(m, l);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -659,67 +670,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         else asm volatile("bar.sync 2, 128;" ::: "memory");
         if (s.last[t]) {
           __threadfence();
-          // A warp joins its 32 rows, 8 at a time: lane r has row r's
-          // statistics, and all lanes HD / 32 columns of every row, so that 8
-          // loads are in flight for each piece.
-          constexpr int kC = HD / 32;
-          const int w0 = (warp & 3) * 32;
-          const float* src0 = a.partial + (long long)(t * 128 + w0) * kLd;
-          const long long slot_f = 256ll * kLd;
+          auto at = [&](int k) { return part0 + paged_slot(p.first_cta + k, p.first_cta) * slot_f; };
+          auto stat = [&](int k) { return __ldcg(reinterpret_cast<const float2*>(at(k) + 128 * HD + 2 * row)); };
           float mm = -INFINITY, ll = 0.f;
-          if (valid)
-            for (int k = 0; k < p.n_ctas; ++k)
-              mm = fmaxf(mm, __ldcg(src0 + paged_slot(p.first_cta + k, p.first_cta) * slot_f + lane * kLd));
-          const float b = mm == -INFINITY ? 0.f : mm;
-#pragma unroll 1
-          for (int r0 = 0; r0 < 32; r0 += 8) {
-            float acc[8][kC];
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-#pragma unroll
-              for (int c = 0; c < kC; ++c) acc[r][c] = 0.f;
-            ll = 0.f;
-#pragma unroll 1
+          if (valid) {
+#pragma unroll 8
+            for (int k = 0; k < p.n_ctas; ++k) mm = fmaxf(mm, stat(k).x);
+            const float b = mm == -INFINITY ? 0.f : mm;
+#pragma unroll 4
             for (int k = 0; k < p.n_ctas; ++k) {
-              const float* src = src0 + paged_slot(p.first_cta + k, p.first_cta) * slot_f;
-              float4 v[8];
-#pragma unroll
-              for (int r = 0; r < 8; ++r) {
-                v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (w0 + r0 + r < rows) {
-                  const float* at = src + (r0 + r) * kLd + 4 + lane * kC;
-                  if constexpr (kC == 4) {
-                    v[r] = __ldcg(reinterpret_cast<const float4*>(at));
-                  } else {
-                    const float2 h = __ldcg(reinterpret_cast<const float2*>(at));
-                    v[r].x = h.x, v[r].y = h.y;
-                  }
-                }
-              }
-              float2 ml = make_float2(-INFINITY, 0.f);
-              if (valid) ml = __ldcg(reinterpret_cast<const float2*>(src + lane * kLd));
-              const float g = ml.y == 0.f ? 0.f : paged_exp2(ml.x - b);
-              ll += ml.y * g;
-#pragma unroll
-              for (int r = 0; r < 8; ++r) {
-                const float gr = __shfl_sync(0xffffffffu, g, r0 + r);
-                acc[r][0] += v[r].x * gr, acc[r][1] += v[r].y * gr;
-                if constexpr (kC == 4) acc[r][2] += v[r].z * gr, acc[r][3] += v[r].w * gr;
-              }
+              const float2 ml = stat(k);
+              ll += ml.y == 0.f ? 0.f : ml.y * paged_exp2(ml.x - b);
             }
             const float iv = see > 0 ? 1.0f / ll : 0.f;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+              float o[32];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-              const int rr = w0 + r0 + r;
-              const float ir = __shfl_sync(0xffffffffu, iv, r0 + r);
-              if (rr >= rows) continue;
-              T* out = static_cast<T*>(a.out) + (p.req.q0 + t0 + t * tile_tokens + rr / a.group) * a.out_stride +
-                       (long long)(p.h * a.group + rr % a.group) * HD + lane * kC;
-              if constexpr (kC == 4)
-                *reinterpret_cast<uint2*>(out) = make_uint2(Frag<T>::pack(acc[r][0] * ir, acc[r][1] * ir),
-                                                            Frag<T>::pack(acc[r][2] * ir, acc[r][3] * ir));
-              else
-                *reinterpret_cast<uint32_t*>(out) = Frag<T>::pack(acc[r][0] * ir, acc[r][1] * ir);
+              for (int j = 0; j < 32; ++j) o[j] = 0.f;
+#pragma unroll 2
+              for (int k = 0; k < p.n_ctas; ++k) {
+                const float2 ml = stat(k);
+                float4 v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = __ldcg(reinterpret_cast<const float4*>(at(k) + ((c / 4 + j) * 128 + row) * 4));
+                const float g = ml.y == 0.f ? 0.f : paged_exp2(ml.x - b);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  o[4 * j] += v[j].x * g, o[4 * j + 1] += v[j].y * g, o[4 * j + 2] += v[j].z * g, o[4 * j + 3] += v[j].w * g;
+              }
+              store(c, o, iv);
             }
           }
           if (valid && a.lse)
