@@ -8,7 +8,11 @@
 // buffers, so Q K^T of the next step runs while the softmax of this one does:
 // with one buffer of 128 keys the chain softmax -> P V -> Q K^T took 4070
 // cycles per 128 keys, of which the tensor cores worked 2048.  64 keys cost
-// shared-memory bandwidth (Q is read again for each), about 2560 cycles.
+// shared-memory bandwidth (Q is read again for each), about 2560 cycles per 128
+// keys.  Now a step of both tiles takes about 1930 cycles (1280 of MMAs, 1024
+// of exponentials): 4 chunks of up to 2048 tokens behind up to 16,384 keys (32
+// heads, 8 K/V heads of 128, bf16) take 1.44 to 1.7 ms with the clock, up to
+// 960 TFLOP/s.  The softmax's latency, one thread per row, is what is left.
 // Roles: warps 0-3 and 4-7 are the softmax of tile 0 and 1, warps 8 and 9 issue
 // their MMAs (in step i P V (i), then Q K^T (i + 2) into the buffer that P was
 // in; the queue of MMAs is short, and one thread's waits for both tiles left
